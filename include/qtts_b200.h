@@ -313,6 +313,127 @@ int32_t qtts_last_launch_count(const qtts_engine* engine, size_t* kernels);
 int32_t qtts_profile_projection(qtts_engine* engine, int32_t which, int32_t launches,
                                 float* ms_per_launch, double* bytes_per_launch);
 
+/* ---------------------------------------------------------------------------
+ * Paged key / value caches in caller-owned device memory (no reference
+ * counterpart; the engine's own talker cache has the same page layout). For
+ * hosts that run their own attention layers or schedule many sequences:
+ * store rows, attend to them (all positions, or a sliding window plus first
+ * positions that stay visible), and fork, free, evict and compact pages.
+ *
+ * Position p of sequence s is row p % page_size of page
+ * page_table[s * max_pages + p / page_size]; -1 names no page. A page holds
+ * one tile of page_size rows for every (layer, K or V, kv head), in that
+ * order; head_dim is 128.
+ *   bits 16: rows of 128 bf16.
+ *   bits 4:  rows of 64 code bytes, then (after the tile's last code row) rows
+ *            of four bf16 scales, one for each 32 dims. 32-bit word 4 t + g of
+ *            a row's codes holds dims 32 g + 8 t .. + 7, lowest nibble first; a
+ *            code is n + 8 with n in -7 .. 7, value n * scale. Storing takes
+ *            scale = bf16(largest magnitude / 7) and n = x / scale, each rounded
+ *            once to nearest (ties to even). A group with a non-finite value
+ *            gets a NaN scale. 72 bytes a row instead of 256.
+ * refs[p] counts the table entries that name page p; 0: the page is free.
+ * An empty cache has page_table all -1, lengths and refs 0.
+ *
+ * Every pointer of these two structs is device memory of `device`, and every
+ * call but qtts_kv_check only enqueues kernels on `stream` (a cudaStream_t of
+ * that device; NULL: the legacy default stream): no allocation, no wait, and
+ * all of them may be captured into a CUDA graph (lists and lengths passed
+ * from the host are fixed at capture). The current device is left as it was.
+ * Calls on one cache must be ordered by the caller (one stream, or events).
+ * `work` is scratch of the page-management calls plus the status word: an
+ * array of qtts_kv_sizes() ints, zeroed once by the caller.
+ */
+typedef enum {
+  QTTS_F32 = 0,
+  QTTS_BF16 = 1,
+} qtts_dtype;
+
+typedef struct {
+  void* pool;          /* pages * page bytes (qtts_kv_sizes), 16-byte aligned */
+  int32_t* page_table; /* [seqs][max_pages]                                   */
+  int32_t* lengths;    /* [seqs] positions held                               */
+  int32_t* refs;       /* [pages]; may be NULL for append, read and attend    */
+  int32_t* work;
+  int32_t device;
+  int32_t pages;
+  int32_t seqs;
+  int32_t max_pages;   /* page-table entries of a sequence                    */
+  int32_t layers;
+  int32_t kv_heads;
+  int32_t page_size;   /* 16, 32, 64, 128 or 256                              */
+  int32_t bits;        /* 16 or 4                                             */
+} qtts_kv_cache;
+
+/* Which rows of a call belong to which sequence: group i is the rows
+ * row_start[i] .. row_start[i + 1] - 1 of sequence seqs[i], its LAST rows in
+ * order (row j of r is position length - r + j: lengths already count them).
+ * Rows outside every group are left as they are. */
+typedef struct {
+  const int32_t* seqs;      /* device [groups]; NULL: sequence i              */
+  const int32_t* row_start; /* device [groups + 1]; NULL: one row each        */
+  int32_t groups;
+  int32_t rows;             /* rows of the tensors                            */
+  int32_t max_rows;         /* most rows of a group, 0: unknown (speed only)  */
+  int32_t max_length;       /* longest sequence, 0: unknown (speed only)      */
+} qtts_kv_rows;
+
+/* Bytes of `pool` and ints of `work` that the cache's other fields call for
+ * (its pointers are not looked at). */
+int32_t qtts_kv_sizes(const qtts_kv_cache* cache, size_t* pool_bytes, size_t* work_ints);
+/* Stores the rows' keys and values [rows][kv_heads][128] (strides in elements,
+ * the last dim contiguous) in `layer`. The pages must not be shared (resize
+ * sees to that for the positions it adds). Of a sequence named by two groups
+ * the last group's rows are stored. */
+int32_t qtts_kv_append(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows,
+                       const void* k, size_t k_row, size_t k_head, const void* v, size_t v_row,
+                       size_t v_head, int32_t dtype, void* stream);
+/* The reverse: what the cache holds for these rows; zeros where it has no page. */
+int32_t qtts_kv_read(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows, void* k,
+                     size_t k_row, size_t k_head, void* v, size_t v_row, size_t v_head,
+                     int32_t dtype, void* stream);
+/* out[row][h] = sum over the keys c that the row sees of
+ * softmax_c(scale * q[row][h] . k_c) * v_c, q head h on kv head
+ * h / (q_heads / kv_heads). The row at position p sees c <= p with
+ * p - c < window, or c < sinks; window 0: every c <= p. Positions without a
+ * page are not seen; a row that sees nothing gives zeros. q and out are
+ * [rows][q_heads][128]; out must not overlap q. Scores, statistics and sums
+ * are fp32; out is rounded once. Repeated calls give the same bits. */
+int32_t qtts_kv_attend(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows,
+                       const void* q, size_t q_row, size_t q_head, void* out, size_t out_row,
+                       size_t out_head, int32_t dtype, int32_t q_heads, float scale,
+                       int32_t window, int32_t sinks, void* stream);
+
+/* Page management. Lists are host arrays (at most 1024 sequences, none
+ * twice). Free pages are handed out lowest index first, in the order of the
+ * list. A call that finds too few changes nothing and records it in the
+ * status word (qtts_kv_check).
+ * resize: sequence seqs[i] gets lengths[i] positions. Pages past the end are
+ *   given back, missing ones taken; a sequence that grows out of a partly
+ *   filled page that it shares gets its own copy of it first. The new
+ *   positions' contents are undefined until stored.
+ * fork: sequence dst[i] becomes a copy of src[i] (several may share a source;
+ *   no source is a destination). What dst held is given back; full pages are
+ *   shared, a partly filled last page is copied.
+ * free: the sequences become empty.
+ * evict: gives back the pages that rows at or after the newest position do
+ *   not see under (window, sinks); lengths stay.
+ * compact: the n pages in use move to indices 0 .. n - 1: those at n or above,
+ *   in order, to the free ones below, in order. Tables follow. */
+int32_t qtts_kv_resize(const qtts_kv_cache* cache, const int32_t* seqs, const int32_t* lengths,
+                       size_t n, void* stream);
+int32_t qtts_kv_fork(const qtts_kv_cache* cache, const int32_t* src, const int32_t* dst, size_t n,
+                     void* stream);
+int32_t qtts_kv_free(const qtts_kv_cache* cache, const int32_t* seqs, size_t n, void* stream);
+int32_t qtts_kv_evict(const qtts_kv_cache* cache, const int32_t* seqs, size_t n, int32_t window,
+                      int32_t sinks, void* stream);
+int32_t qtts_kv_compact(const qtts_kv_cache* cache, void* stream);
+/* Waits for `stream`, then returns and clears the status word:
+ * QTTS_ERR_CACHE_FULL after a resize or fork that found too few pages,
+ * QTTS_ERR_DEVICE_STATE after a table entry, sequence, length or row count
+ * out of range (what it concerned was skipped). Not during capture. */
+int32_t qtts_kv_check(const qtts_kv_cache* cache, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,194 @@
+"""The paged key / value cache in plain Python: 64-bit attention row by row,
+the 4-bit format in exact arithmetic, and the page bookkeeping as loops.
+
+TEST INFRASTRUCTURE: the GPU kernels of ``qtts_kv_*`` are compared with this.
+"""
+from __future__ import annotations
+
+from fractions import Fraction
+
+import numpy as np
+
+DIM, GROUP = 128, 32
+
+
+def nearest_even(x: Fraction) -> int:
+    f = x.numerator // x.denominator
+    r = x - f
+    if r > Fraction(1, 2) or (r == Fraction(1, 2) and f % 2):
+        f += 1
+    return f
+
+
+def bf16_of(x: Fraction) -> float:
+    """x >= 0 rounded once to bf16 (ties to even), subnormals included."""
+    if x == 0:
+        return 0.0
+    e = -133  # exponent of the last place: bf16 subnormals are multiples of 2^-133
+    while x >= Fraction(2) ** (e + 8):
+        e += 1
+    return float(nearest_even(x / Fraction(2) ** e) * Fraction(2) ** e)
+
+
+def quantise_row(x) -> tuple:
+    """128 float32 values -> (n int [128], scale float [4]); a group with a
+    non-finite value has a NaN scale and n = 0."""
+    x = np.asarray(x, dtype=np.float32)
+    n, s = np.zeros(DIM, np.int64), np.zeros(DIM // GROUP)
+    for g in range(DIM // GROUP):
+        part = x[g * GROUP: (g + 1) * GROUP]
+        if not np.isfinite(part).all():
+            s[g] = np.nan
+            continue
+        top = Fraction(float(np.abs(part).max()))
+        s[g] = bf16_of(top / 7)
+        if s[g] > 0:
+            for i, v in enumerate(part):
+                q = nearest_even(abs(Fraction(float(v))) / Fraction(s[g]))
+                n[g * GROUP + i] = (1 if v > 0 else -1) * min(q, 7)
+    return n, s
+
+
+def quantise_fast(x: np.ndarray) -> np.ndarray:
+    """Values [.., 128] that the cache holds for x: float64 quotients, whose
+    rounding matches the exact one (a float32 over a bf16 or over 7 is never
+    within 2^-50 of a border without being on it)."""
+    g = x.astype(np.float64).reshape(-1, GROUP)
+    m, e = np.frexp(np.abs(g).max(1, keepdims=True) / 7.0)
+    s = np.ldexp(np.rint(np.ldexp(m, 8)), e - 8)
+    n = np.clip(np.rint(np.divide(g, s, out=np.zeros_like(g), where=s > 0)), -7, 7)
+    return (n * s).reshape(x.shape)
+
+
+def code_place(d: int) -> tuple:
+    """(byte, shift) of dim d in a row's 64 code bytes."""
+    t, g = (d % 32) // 8, d // 32
+    nib = d % 8
+    return 4 * (4 * t + g) + nib // 2, 4 * (nib % 2)
+
+
+def sees(pos: int, key: int, window: int, sinks: int) -> bool:
+    return key <= pos and (window == 0 or pos - key < window or key < sinks)
+
+
+def attend(q, keys, values, held, pos, window, sinks, scale):
+    """One row: q [heads, 128], keys / values [length, kv heads, 128] float64,
+    held [length] bool. Zeros when nothing is seen."""
+    heads, kv = q.shape[0], keys.shape[1]
+    out = np.zeros((heads, DIM))
+    at = [c for c in range(min(pos + 1, len(held))) if held[c] and sees(pos, c, window, sinks)]
+    if not at:
+        return out
+    for h in range(heads):
+        k, v = keys[at, h // (heads // kv)], values[at, h // (heads // kv)]
+        s = (k @ q[h].astype(np.float64)) * scale
+        w = np.exp(s - s.max())
+        out[h] = (w / w.sum()) @ v
+    return out
+
+
+class Cache:
+    """Tables, reference counts and page contents (`data[page]`: any value)."""
+
+    def __init__(self, pages, seqs, max_pages, page_size):
+        self.ps = page_size
+        self.table = [[-1] * max_pages for _ in range(seqs)]
+        self.lengths = [0] * seqs
+        self.refs = [0] * pages
+        self.data = [None] * pages
+
+    def need(self, n):
+        return -(-n // self.ps)
+
+    def free_pages(self):
+        return [p for p, r in enumerate(self.refs) if r == 0]
+
+    def _snapshot(self):
+        return [list(r) for r in self.table], list(self.lengths), list(self.refs), list(self.data)
+
+    def _restore(self, s):
+        self.table, self.lengths, self.refs, self.data = s
+
+    def _give(self, s, j):
+        p = self.table[s][j]
+        if p >= 0:
+            self.refs[p] -= 1
+            self.table[s][j] = -1
+
+    def resize(self, seqs, lengths) -> bool:
+        was = self._snapshot()
+        for s, n in zip(seqs, lengths):
+            for j in range(self.need(n), len(self.table[s])):
+                self._give(s, j)
+        wants = []
+        for s, n in zip(seqs, lengths):
+            old = self.lengths[s]
+            if n <= old:
+                continue
+            for j in range(old // self.ps, self.need(n)):
+                p = self.table[s][j]
+                shared = j == old // self.ps and old % self.ps and p >= 0 and self.refs[p] > 1
+                if p < 0 or shared:
+                    wants.append((s, j, p if shared else -1))
+        free = self.free_pages()
+        if len(free) < len(wants):
+            self._restore(was)
+            return False
+        for (s, j, p), new in zip(wants, free):
+            if p >= 0:
+                self.refs[p] -= 1
+                self.data[new] = self.data[p]
+            self.table[s][j] = new
+            self.refs[new] = 1
+        for s, n in zip(seqs, lengths):
+            self.lengths[s] = n
+        return True
+
+    def fork(self, src, dst) -> bool:
+        was = self._snapshot()
+        for d in dst:
+            for j in range(len(self.table[d])):
+                self._give(d, j)
+        wants = []
+        for s, d in zip(src, dst):
+            n = self.lengths[s]
+            if n % self.ps and self.table[s][n // self.ps] >= 0:
+                wants.append((s, d, n // self.ps))
+        free = self.free_pages()
+        if len(free) < len(wants):
+            self._restore(was)
+            return False
+        for s, d in zip(src, dst):
+            for j in range(self.lengths[s] // self.ps):
+                p = self.table[s][j]
+                self.table[d][j] = p
+                if p >= 0:
+                    self.refs[p] += 1
+            self.lengths[d] = self.lengths[s]
+        for (s, d, j), new in zip(wants, free):
+            self.table[d][j] = new
+            self.refs[new] = 1
+            self.data[new] = self.data[self.table[s][j]]
+        return True
+
+    def free(self, seqs):
+        for s in seqs:
+            for j in range(len(self.table[s])):
+                self._give(s, j)
+            self.lengths[s] = 0
+
+    def evict(self, seqs, window, sinks):
+        for s in seqs:
+            for j in range(len(self.table[s])):
+                first, end = j * self.ps, (j + 1) * self.ps
+                if first >= sinks and end <= self.lengths[s] - window:
+                    self._give(s, j)
+
+    def compact(self):
+        n = sum(r > 0 for r in self.refs)
+        src = [p for p in range(n, len(self.refs)) if self.refs[p] > 0]
+        dst = [p for p in range(n) if self.refs[p] == 0]
+        to = dict(zip(src, dst))
+        for s, d in to.items():
+            self.data[d], self.refs[d], self.refs[s] = self.data[s], self.refs[s], 0
+        self.table = [[to.get(p, p) for p in row] for row in self.table]

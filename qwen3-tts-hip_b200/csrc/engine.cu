@@ -30,29 +30,20 @@
 #include <vector>
 
 #include "codec.h"
+#include "error.h"
 #include "gemm_tc.h"
 #include "json.h"
 #include "kernels.h"
 #include "qtts_b200.h"
 
 namespace qtts {
+
+std::string& last_error() {
+  thread_local std::string message;
+  return message;
+}
+
 namespace {
-
-thread_local std::string g_last_error;
-
-struct QttsError : std::runtime_error {
-  int code;
-  QttsError(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-[[noreturn]] void fail(int code, const std::string& m) { throw QttsError(code, m); }
-[[noreturn]] void invalid(const std::string& m) { fail(QTTS_ERR_INVALID_INPUT, m); }
-
-#define QCK(expr)                                                                     \
-  do {                                                                                \
-    cudaError_t e_ = (expr);                                                          \
-    if (e_ != cudaSuccess)                                                            \
-      ::qtts::fail(QTTS_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
-  } while (0)
 
 constexpr uint64_t kSeedXor = 0x9e3779b97f4a7c15ull;  // generation.rs:667
 constexpr int kNewline = 198;                          // text.rs:15
@@ -2173,6 +2164,8 @@ struct TextStream {
 }  // namespace qtts
 
 using qtts::Engine;
+using qtts::guard;
+using qtts::need;
 using qtts::QttsError;
 
 struct qtts_engine {
@@ -2190,27 +2183,6 @@ struct qtts_codec_stream {
 };
 
 namespace {
-
-template <typename F>
-int32_t guard(F&& f) {
-  try {
-    f();
-    return QTTS_OK;
-  } catch (const QttsError& e) {
-    qtts::g_last_error = e.what();
-    return e.code;
-  } catch (const std::bad_alloc&) {
-    qtts::g_last_error = "out of host memory";
-    return QTTS_ERR_CUDA;
-  } catch (const std::exception& e) {
-    qtts::g_last_error = e.what();
-    return QTTS_ERR_INVALID_INPUT;
-  }
-}
-
-void need(const void* p, const char* what) {
-  if (!p) qtts::invalid(std::string(what) + " must not be null");
-}
 
 Engine& engine_of(qtts_engine* e) {
   need(e, "engine");
@@ -2262,7 +2234,7 @@ long long next_trailing_id(qtts::TextStream& s) {
 
 extern "C" {
 
-const char* qtts_last_error(void) { return qtts::g_last_error.c_str(); }
+const char* qtts_last_error(void) { return qtts::last_error().c_str(); }
 int32_t qtts_abi_version(void) { return 2; }
 
 void qtts_generate_options_default(qtts_generate_options* o) {
@@ -2306,7 +2278,7 @@ int32_t qtts_engine_load(const char* dir, int32_t device, qtts_engine** out) {
 int32_t qtts_engine_load_with_max_frames(const char* dir, int32_t device, size_t max_frames,
                                          qtts_engine** out) {
   if (max_frames == 0) {
-    qtts::g_last_error = "max_frames must be non-zero";
+    qtts::last_error() = "max_frames must be non-zero";
     return QTTS_ERR_INVALID_INPUT;
   }
   return load_engine(dir, device, 256 + max_frames, out);

@@ -1,0 +1,164 @@
+// Device helpers of the paged key / value cache kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "kv.h"
+
+namespace qtts {
+
+__device__ __forceinline__ void kv_status(const KvArgs& c, int bit) {
+  if (c.work) atomicOr(c.work, bit);
+}
+__device__ __forceinline__ void kv_bad(const KvArgs& c) { kv_status(c, kKvBadIndex); }
+
+__device__ __forceinline__ int kv_length(const KvArgs& c, int seq) {
+  return c.lengths ? __ldcg(c.lengths + (long long)seq * c.len_stride) + c.len_add : c.len_add;
+}
+
+// Physical page of a sequence's logical page, or -1: no page, or a table
+// entry that names none (recorded). Callers keep `logical` below max_pages.
+__device__ __forceinline__ int kv_page(const KvArgs& c, int seq, int logical) {
+  const int p = __ldcg(c.table + (long long)seq * c.g.max_pages + logical);
+  if ((unsigned)p < (unsigned)c.g.pages) return p;
+  if (p != -1) kv_bad(c);
+  return -1;
+}
+
+// Where a row belongs: its group (-1: to none; it is left alone), sequence and
+// position. ok: the position is one a sequence can hold. Warp-collective.
+struct KvPlace {
+  int group, seq, pos;
+  bool ok;
+};
+__device__ __forceinline__ KvPlace kv_place(const KvArgs& c, const KvRows& r, int row, bool write) {
+  const int lane = threadIdx.x & 31;
+  KvPlace at{-1, 0, -1, false};
+  int back = 1;  // rows from this one to the group's last
+  if (r.row_start) {
+    // groups that end at or before this row
+    int before = 0;
+    for (int i = lane; i < r.groups; i += 32) before += __ldg(r.row_start + i + 1) <= row;
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (before >= r.groups || row < __ldg(r.row_start + before)) return at;
+    at.group = before;
+    back = __ldg(r.row_start + before + 1) - row;
+  } else {
+    if (row >= r.groups) return at;
+    at.group = row;
+  }
+  at.seq = r.seqs ? __ldg(r.seqs + at.group) : at.group;
+  if ((unsigned)at.seq >= (unsigned)c.g.seqs) {
+    kv_bad(c);
+    return at;
+  }
+  if (write && r.seqs) {
+    // of a sequence that is named twice, the last group's rows are stored
+    int later = 0;
+    for (int i = at.group + 1 + lane; i < r.groups; i += 32) later |= __ldg(r.seqs + i) == at.seq;
+    if (__any_sync(0xffffffffu, later)) return at;
+  }
+  const int len = kv_length(c, at.seq);
+  if (len < 0 || len > kv_capacity(c.g)) {
+    kv_bad(c);
+    return at;
+  }
+  at.pos = len - back;
+  at.ok = at.pos >= 0 && back > 0;
+  if (back <= 0 || (write && at.pos < 0)) kv_bad(c);
+  return at;
+}
+
+// Four consecutive values of a row tensor; 16-byte (8-byte) accesses where the
+// address allows, else one by one.
+__device__ __forceinline__ float4 kv_load4(const void* p, long long off, int type) {
+  if (type == KV_F32) {
+    const float* f = static_cast<const float*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) return __ldcg(reinterpret_cast<const float4*>(f));
+    return make_float4(f[0], f[1], f[2], f[3]);
+  }
+  const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p) + off;
+  if ((reinterpret_cast<uintptr_t>(b) & 7) == 0) {
+    const uint2 u = __ldcg(reinterpret_cast<const uint2*>(b));
+    return make_float4(bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y));
+  }
+  return make_float4(__bfloat162float(b[0]), __bfloat162float(b[1]), __bfloat162float(b[2]),
+                     __bfloat162float(b[3]));
+}
+__device__ __forceinline__ void kv_store4(void* p, long long off, int type, float4 v) {
+  if (type == KV_F32) {
+    float* f = static_cast<float*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) {
+      *reinterpret_cast<float4*>(f) = v;
+    } else {
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    }
+    return;
+  }
+  __nv_bfloat16* b = static_cast<__nv_bfloat16*>(p) + off;
+  const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+  if ((reinterpret_cast<uintptr_t>(b) & 7) == 0) {
+    *reinterpret_cast<uint2*>(b) = make_uint2(*reinterpret_cast<const unsigned*>(&x),
+                                              *reinterpret_cast<const unsigned*>(&y));
+  } else {
+    b[0] = x.x; b[1] = x.y; b[2] = y.x; b[3] = y.y;
+  }
+}
+
+// Dims 4 lane .. 4 lane + 3 of a cached row.
+__device__ __forceinline__ float4 kv_cached4(const KvArgs& c, int page, int layer, int which,
+                                             int head, int row, int lane) {
+  const unsigned char* tile = c.pool + kv_tile_at(c.g, page, layer, which, head);
+  const unsigned char* cell = tile + kv_row_at(c.g, row);
+  if (c.g.bits == 16) {
+    const uint2 u = *(reinterpret_cast<const uint2*>(cell) + lane);
+    return make_float4(bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y));
+  }
+  const unsigned n = *(reinterpret_cast<const uint16_t*>(cell + kv_code_word_at(4 * lane)) + (lane & 1));
+  const float s = __bfloat162float(
+      *(reinterpret_cast<const __nv_bfloat16*>(tile + kv_scale_at(c.g, row)) + (lane >> 3)));
+  return make_float4((float)((int)(n & 15u) - 8) * s, (float)((int)((n >> 4) & 15u) - 8) * s,
+                     (float)((int)((n >> 8) & 15u) - 8) * s, (float)((int)(n >> 12) - 8) * s);
+}
+
+// Scale of a group from its largest magnitude: amax / 7 rounded once to the
+// nearest bf16 (ties to even). fl(amax / 7) may sit on a bf16 midpoint that
+// the exact quotient only comes near, so the midpoint decides by 7 * mid,
+// which is exact (12 bits). Non-finite: NaN, which marks the group.
+__device__ __forceinline__ float kv_scale_of(float amax) {
+  if (!isfinite(amax)) return __int_as_float(0x7fc00000);
+  const unsigned lo = __float_as_uint(amax / 7.0f) & 0xffff0000u;
+  const float s0 = __uint_as_float(lo), s1 = __uint_as_float(lo + 0x10000u);
+  const float mid7 = 7.0f * (s0 + 0.5f * (s1 - s0));
+  return amax > mid7 || (amax == mid7 && (lo & 0x10000u)) ? s1 : s0;
+}
+// Code of x: x / s rounded once to the nearest integer (ties to even), limited
+// to -7..7, plus 8. The rounded quotient may sit on a half the exact one does
+// not reach, so (n +- 1/2) * s, exact in fp32 (13 bits), decides.
+__device__ __forceinline__ unsigned kv_code_of(float x, float s) {
+  if (!(s > 0.f)) return 8u;  // all zeros, or a marked group
+  const float a = fabsf(x);
+  float n = fminf(rintf(a / s), 8.0f);
+  const float up = (n + 0.5f) * s, dn = (n - 0.5f) * s;
+  const bool odd = ((int)n & 1) != 0;
+  if (a > up || (a == up && odd)) n += 1.0f;
+  else if (a < dn || (a == dn && odd)) n -= 1.0f;
+  n = fminf(n, 7.0f);
+  return (unsigned)(8 + (int)(x < 0.f ? -n : n));
+}
+// Warp-collective over the eight lanes of a group: the 16 bits of this lane's
+// four codes, and the group's scale.
+__device__ __forceinline__ unsigned kv_quantise4(float4 x, float* scale) {
+  // a NaN would drop out of fmaxf: it is carried as infinity
+  auto mag = [](float v) { return v == v ? fabsf(v) : __int_as_float(0x7f800000); };
+  float m = fmaxf(fmaxf(mag(x.x), mag(x.y)), fmaxf(mag(x.z), mag(x.w)));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float s = kv_scale_of(m);
+  *scale = s;
+  return kv_code_of(x.x, s) | (kv_code_of(x.y, s) << 4) | (kv_code_of(x.z, s) << 8) |
+         (kv_code_of(x.w, s) << 12);
+}
+
+}  // namespace qtts

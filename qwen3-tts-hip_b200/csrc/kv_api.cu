@@ -1,0 +1,295 @@
+// C entry points of the paged key / value caches (qtts_kv_*): argument
+// checks, then one launch (two for calls that copy pages) on the caller's
+// stream. Nothing here allocates or waits except qtts_kv_check.
+#include <cmath>
+#include <vector>
+
+#include "error.h"
+#include "kv.h"
+
+namespace {
+
+using qtts::guard;
+using qtts::invalid;
+using qtts::need;
+
+// Makes the cache's device current for one call.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    QCK(cudaGetDevice(&old_));
+    if (device != old_) QCK(cudaSetDevice(device));
+    changed_ = device != old_;
+  }
+  ~DeviceScope() {
+    if (changed_) cudaSetDevice(old_);
+  }
+
+ private:
+  int old_ = 0;
+  bool changed_ = false;
+};
+
+qtts::KvGeom geom_of(const qtts_kv_cache* c) {
+  need(c, "cache");
+  auto positive = [](int32_t v, const char* what) {
+    if (v <= 0) invalid(std::string("cache.") + what + " must be positive, got " + std::to_string(v));
+  };
+  positive(c->pages, "pages");
+  positive(c->seqs, "seqs");
+  positive(c->max_pages, "max_pages");
+  positive(c->layers, "layers");
+  positive(c->kv_heads, "kv_heads");
+  if (c->kv_heads > 1024) invalid("cache.kv_heads must be at most 1024");
+  if (c->bits != 16 && c->bits != 4)
+    invalid("cache.bits must be 16 or 4, got " + std::to_string(c->bits));
+  int shift = qtts::kKvMinShift;
+  while (shift <= qtts::kKvMaxShift && (1 << shift) != c->page_size) ++shift;
+  if (shift > qtts::kKvMaxShift)
+    invalid("cache.page_size must be 16, 32, 64, 128 or 256, got " + std::to_string(c->page_size));
+  qtts::KvGeom g{c->pages, c->seqs, c->max_pages, c->layers, c->kv_heads, shift, c->bits};
+  if (qtts::kv_capacity(g) > INT32_MAX) invalid("cache.max_pages * page_size exceeds 2^31 - 1");
+  if ((long long)c->pages > (1LL << 28)) invalid("cache.pages must be at most 2^28");
+  return g;
+}
+
+qtts::KvArgs args_of(const qtts_kv_cache* c, bool managed) {
+  qtts::KvArgs a{};
+  a.g = geom_of(c);
+  need(c->pool, "cache.pool");
+  if (reinterpret_cast<uintptr_t>(c->pool) & 15) invalid("cache.pool must be 16-byte aligned");
+  need(c->page_table, "cache.page_table");
+  need(c->lengths, "cache.lengths");
+  need(c->work, "cache.work");
+  if (managed) need(c->refs, "cache.refs");
+  a.pool = static_cast<unsigned char*>(c->pool);
+  a.table = c->page_table;
+  a.lengths = c->lengths;
+  a.len_stride = 1;
+  a.refs = c->refs;
+  a.work = c->work;
+  return a;
+}
+
+qtts::KvRows rows_of(const qtts_kv_cache* c, const qtts_kv_rows* r) {
+  need(r, "rows");
+  if (r->groups < 0 || r->rows < 0) invalid("rows.groups and rows.rows must not be negative");
+  if (r->max_rows < 0 || r->max_length < 0)
+    invalid("rows.max_rows and rows.max_length must not be negative");
+  if (!r->row_start && r->rows != r->groups)
+    invalid("without row_start each group has one row: rows.rows must equal rows.groups");
+  if (!r->seqs && r->groups > c->seqs)
+    invalid("rows.groups exceeds the cache's sequences and rows.seqs is null");
+  qtts::KvRows k{r->seqs, r->row_start, r->groups, r->groups ? r->rows : 0, r->max_rows,
+                 r->max_length};
+  if (k.max_rows == 0 || k.max_rows > k.rows) k.max_rows = k.row_start ? k.rows : 1;
+  return k;
+}
+
+void check_layer(const qtts_kv_cache* c, int32_t layer) {
+  if (layer < 0 || layer >= c->layers)
+    invalid("layer " + std::to_string(layer) + " is outside the cache's " +
+            std::to_string(c->layers));
+}
+
+qtts::KvTensor tensor_of(const void* p, size_t row, size_t head, int32_t type, int rows,
+                         const char* what) {
+  if (type != QTTS_F32 && type != QTTS_BF16) invalid("dtype must be QTTS_F32 or QTTS_BF16");
+  if (rows) need(p, what);
+  if (reinterpret_cast<uintptr_t>(p) & (type == QTTS_F32 ? 3 : 1))
+    invalid(std::string(what) + " is not aligned to its element type");
+  if (row > (size_t)1 << 40 || head > (size_t)1 << 40) invalid(std::string(what) + ": stride too large");
+  return qtts::KvTensor{const_cast<void*>(p), (long long)row, (long long)head};
+}
+
+// A list of sequences: in range, none twice.
+void put_list(const qtts_kv_cache* c, const int32_t* s, size_t n, const char* what, int* out,
+              std::vector<char>& seen) {
+  if (n > (size_t)qtts::kKvMaxList)
+    invalid("at most " + std::to_string(qtts::kKvMaxList) + " sequences per call");
+  if (n) need(s, what);
+  for (size_t i = 0; i < n; ++i) {
+    if (s[i] < 0 || s[i] >= c->seqs)
+      invalid(std::string(what) + ": sequence " + std::to_string(s[i]) + " is outside the cache's " +
+              std::to_string(c->seqs));
+    if (seen[s[i]]) invalid(std::string(what) + ": sequence " + std::to_string(s[i]) + " is named twice");
+    seen[s[i]] = 1;
+    out[i] = s[i];
+  }
+}
+
+qtts::KvList one_list(const qtts_kv_cache* c, const int32_t* s, size_t n, const char* what) {
+  qtts::KvList l;
+  std::vector<char> seen((size_t)c->seqs);
+  put_list(c, s, n, what, l.a, seen);
+  l.n = (int)n;
+  return l;
+}
+
+cudaStream_t stream_of(void* s) { return static_cast<cudaStream_t>(s); }
+
+void check_span(int32_t window, int32_t sinks) {
+  if (window < 0) invalid("window must not be negative (0: no window)");
+  if (sinks < 0) invalid("sinks must not be negative");
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t qtts_kv_sizes(const qtts_kv_cache* cache, size_t* pool_bytes, size_t* work_ints) {
+  return guard([&] {
+    const qtts::KvGeom g = geom_of(cache);
+    if (pool_bytes) *pool_bytes = (size_t)g.pages * (size_t)qtts::kv_page_bytes(g);
+    if (work_ints) *work_ints = qtts::kv_work_ints(g);
+  });
+}
+
+int32_t qtts_kv_append(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows,
+                       const void* k, size_t k_row, size_t k_head, const void* v, size_t v_row,
+                       size_t v_head, int32_t dtype, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, false);
+    check_layer(cache, layer);
+    const qtts::KvRows r = rows_of(cache, rows);
+    const qtts::KvTensor kt = tensor_of(k, k_row, k_head, dtype, r.rows, "k");
+    const qtts::KvTensor vt = tensor_of(v, v_row, v_head, dtype, r.rows, "v");
+    if (r.rows == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_append(c, r, layer, kt, vt, dtype, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_read(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows, void* k,
+                     size_t k_row, size_t k_head, void* v, size_t v_row, size_t v_head,
+                     int32_t dtype, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, false);
+    check_layer(cache, layer);
+    const qtts::KvRows r = rows_of(cache, rows);
+    const qtts::KvTensor kt = tensor_of(k, k_row, k_head, dtype, r.rows, "k");
+    const qtts::KvTensor vt = tensor_of(v, v_row, v_head, dtype, r.rows, "v");
+    if (r.rows == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_read(c, r, layer, kt, vt, dtype, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_attend(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_rows* rows,
+                       const void* q, size_t q_row, size_t q_head, void* out, size_t out_row,
+                       size_t out_head, int32_t dtype, int32_t q_heads, float scale,
+                       int32_t window, int32_t sinks, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, false);
+    check_layer(cache, layer);
+    const qtts::KvRows r = rows_of(cache, rows);
+    qtts::KvAttend a{};
+    a.q = tensor_of(q, q_row, q_head, dtype, r.rows, "q");
+    a.out = tensor_of(out, out_row, out_head, dtype, r.rows, "out");
+    if (q_heads <= 0 || q_heads % cache->kv_heads != 0)
+      invalid("q_heads must be a positive multiple of the cache's " +
+              std::to_string(cache->kv_heads) + " kv heads, got " + std::to_string(q_heads));
+    if (q_heads > 65535) invalid("q_heads must be at most 65535");
+    if (!std::isfinite(scale)) invalid("scale must be finite");
+    check_span(window, sinks);
+    a.type = dtype;
+    a.q_heads = q_heads;
+    a.scale = scale;
+    a.window = window;
+    a.sinks = sinks;
+    a.layer = layer;
+    if (r.rows == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_attend(c, r, a, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_resize(const qtts_kv_cache* cache, const int32_t* seqs, const int32_t* lengths,
+                       size_t n, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, true);
+    qtts::KvList l = one_list(cache, seqs, n, "seqs");
+    if (n) need(lengths, "lengths");
+    for (size_t i = 0; i < n; ++i) {
+      if (lengths[i] < 0 || lengths[i] > qtts::kv_capacity(c.g))
+        invalid("length " + std::to_string(lengths[i]) + " is outside a sequence's " +
+                std::to_string(qtts::kv_capacity(c.g)) + " positions");
+      l.b[i] = lengths[i];
+    }
+    if (n == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_resize(c, l, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_fork(const qtts_kv_cache* cache, const int32_t* src, const int32_t* dst, size_t n,
+                     void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, true);
+    qtts::KvList l;
+    std::vector<char> seen((size_t)cache->seqs);
+    put_list(cache, dst, n, "dst", l.b, seen);
+    if (n) need(src, "src");
+    for (size_t i = 0; i < n; ++i) {
+      if (src[i] < 0 || src[i] >= cache->seqs)
+        invalid("src: sequence " + std::to_string(src[i]) + " is outside the cache's " +
+                std::to_string(cache->seqs));
+      if (seen[src[i]])
+        invalid("src: sequence " + std::to_string(src[i]) + " is also a destination");
+      l.a[i] = src[i];
+    }
+    l.n = (int)n;
+    if (n == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_fork(c, l, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_free(const qtts_kv_cache* cache, const int32_t* seqs, size_t n, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, true);
+    const qtts::KvList l = one_list(cache, seqs, n, "seqs");
+    if (n == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_drop(c, l, -1, 0, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_evict(const qtts_kv_cache* cache, const int32_t* seqs, size_t n, int32_t window,
+                      int32_t sinks, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, true);
+    const qtts::KvList l = one_list(cache, seqs, n, "seqs");
+    check_span(window, sinks);
+    if (window == 0) invalid("evict needs a window");
+    if (n == 0) return;
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_drop(c, l, window, sinks, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_compact(const qtts_kv_cache* cache, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, true);
+    DeviceScope on(cache->device);
+    QCK(qtts::launch_kv_compact(c, stream_of(stream)));
+  });
+}
+
+int32_t qtts_kv_check(const qtts_kv_cache* cache, void* stream) {
+  return guard([&] {
+    const qtts::KvArgs c = args_of(cache, false);
+    DeviceScope on(cache->device);
+    int status = 0;
+    QCK(cudaMemcpyAsync(&status, c.work, sizeof status, cudaMemcpyDeviceToHost, stream_of(stream)));
+    QCK(cudaStreamSynchronize(stream_of(stream)));
+    if (!status) return;
+    QCK(cudaMemsetAsync(c.work, 0, sizeof status, stream_of(stream)));
+    if (status & qtts::kKvBadIndex)
+      qtts::fail(QTTS_ERR_DEVICE_STATE,
+                 "a sequence, length, row or page of the cache was out of range and was skipped");
+    qtts::fail(QTTS_ERR_CACHE_FULL, "too few free pages: the call changed nothing");
+  });
+}
+
+}  // extern "C"

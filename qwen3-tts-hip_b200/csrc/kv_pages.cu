@@ -1,0 +1,364 @@
+// Page management of the paged key / value caches, on the device: the tables,
+// lengths and reference counts never visit the host, so the calls are ordered
+// by their stream and may be captured.
+//
+// refs[p] counts the table entries that name page p; a page with none is
+// free. Pages are handed out lowest index first, in the order of the request
+// list and of its logical pages, so every call is deterministic (the counts
+// are integers: the order of their atomics does not show).
+#include "common.cuh"
+#include "kv.cuh"
+
+namespace qtts {
+
+// work: [0] status, [1] copies listed, then the listed source and destination
+// pages, then one entry per page (free pages found / new place of a page).
+constexpr int kKvWorkHead = 16;
+
+size_t kv_work_ints(const KvGeom& g) {
+  return kKvWorkHead + 2 * (size_t)(g.pages > kKvMaxList ? g.pages : kKvMaxList) + (size_t)g.pages;
+}
+
+namespace {
+
+struct Work {
+  int *copies, *src, *dst, *map;
+};
+__device__ __forceinline__ Work work_of(const KvArgs& c) {
+  const int n = max(c.g.pages, kKvMaxList);
+  int* p = c.work + kKvWorkHead;
+  return Work{c.work + 1, p, p + n, p + 2 * n};
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive prefix of v over the block; *total the sum.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int s_warp[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += n;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int w = s_warp[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += n;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, warp) - __shfl_sync(0xffffffffu, inc, 31);
+  return before + inc - v;
+}
+
+// The lowest `want` free pages in work.map; false when there are fewer.
+__device__ __forceinline__ bool find_free(const KvArgs& c, const Work& w, int want) {
+  int found = 0;
+  for (int p0 = 0; p0 < c.g.pages && found < want; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int is = p < c.g.pages && __ldcg(c.refs + p) <= 0;
+    int total;
+    const int at = found + block_scan(is, &total);
+    if (is && at < want) w.map[at] = p;
+    found += total;
+  }
+  __syncthreads();
+  return found >= want;
+}
+
+__device__ __forceinline__ int table_page(const KvArgs& c, int seq, int j) {
+  return kv_page(c, seq, j);
+}
+__device__ __forceinline__ int checked_length(const KvArgs& c, int seq) {
+  const int n = __ldcg(c.lengths + seq);
+  if (n < 0 || n > kv_capacity(c.g)) {
+    kv_bad(c);
+    return 0;
+  }
+  return n;
+}
+
+// Sequence l.a[i] gets length l.b[i]: entries past its last page are dropped,
+// missing pages are taken, and a tail page that it shares and is going to
+// write into is replaced by a copy (listed for k_copy_pages). One block: the
+// work is a few table rows and a scan of refs.
+__global__ void __launch_bounds__(kPlanThreads) k_resize(KvArgs c, const __grid_constant__ KvList l) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int s_need[kKvMaxList], s_tail[kKvMaxList];
+  const Work w = work_of(c);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kW = kPlanThreads / 32;
+  const int ps = 1 << c.g.shift;
+  auto pages_of = [&](int n) { return (n + ps - 1) >> c.g.shift; };
+  // entries past the new end give their pages back (the table follows once
+  // the call is known to go through)
+  for (int i = warp; i < l.n; i += kW)
+    for (int j = pages_of(l.b[i]) + lane; j < c.g.max_pages; j += 32) {
+      const int p = table_page(c, l.a[i], j);
+      if (p >= 0) atomicSub(c.refs + p, 1);
+    }
+  __syncthreads();
+  // what each sequence is short of; the shared tail page counts as missing
+  for (int i = warp; i < l.n; i += kW) {
+    const int old = checked_length(c, l.a[i]);
+    int need = 0, tail = -1;
+    if (l.b[i] > old) {
+      if (old & (ps - 1)) {
+        const int j = old >> c.g.shift;
+        const int p = table_page(c, l.a[i], j);
+        if (p >= 0 && __ldcg(c.refs + p) > 1) tail = j;
+      }
+      int mine = 0;
+      for (int j = (old >> c.g.shift) + lane; j < pages_of(l.b[i]); j += 32)
+        mine += j == tail || table_page(c, l.a[i], j) < 0;
+      need = __reduce_add_sync(0xffffffffu, mine);
+    }
+    if (lane == 0) {
+      s_need[i] = need;
+      s_tail[i] = tail;
+    }
+  }
+  __syncthreads();
+  int total;
+  const int base = block_scan(threadIdx.x < l.n ? s_need[threadIdx.x] : 0, &total);
+  const bool ok = find_free(c, w, total);
+  if (!ok) {  // everything back as it was
+    for (int i = warp; i < l.n; i += kW)
+      for (int j = pages_of(l.b[i]) + lane; j < c.g.max_pages; j += 32) {
+        const int p = table_page(c, l.a[i], j);
+        if (p >= 0) atomicAdd(c.refs + p, 1);
+      }
+    if (threadIdx.x == 0) {
+      *w.copies = 0;
+      kv_status(c, kKvOutOfPages);
+    }
+    return;
+  }
+  int copies;
+  const int my_copy =
+      block_scan(threadIdx.x < l.n && s_tail[threadIdx.x] >= 0 ? 1 : 0, &copies);
+  if (threadIdx.x < l.n) {
+    s_need[threadIdx.x] = base;  // first entry of this sequence in work.map
+    if (s_tail[threadIdx.x] >= 0) {
+      // the tail is the sequence's first missing page
+      const int i = threadIdx.x, seq = l.a[i], page = w.map[base];
+      const int shared = table_page(c, seq, s_tail[i]);
+      w.src[my_copy] = shared;
+      w.dst[my_copy] = page;
+      atomicSub(c.refs + shared, 1);
+    }
+  }
+  if (threadIdx.x == 0) *w.copies = copies;
+  __syncthreads();
+  for (int i = warp; i < l.n; i += kW) {
+    const int seq = l.a[i], n = l.b[i], old = checked_length(c, seq);
+    int* row = c.table + (long long)seq * c.g.max_pages;
+    for (int j = pages_of(n) + lane; j < c.g.max_pages; j += 32) row[j] = -1;
+    if (n > old) {
+      int at = s_need[i];
+      for (int j0 = old >> c.g.shift; j0 < pages_of(n); j0 += 32) {
+        const int j = j0 + lane;
+        const bool take = j < pages_of(n) && (j == s_tail[i] || table_page(c, seq, j) < 0);
+        const unsigned b = __ballot_sync(0xffffffffu, take);
+        if (take) {
+          const int page = w.map[at + __popc(b & ((1u << lane) - 1u))];
+          row[j] = page;
+          c.refs[page] = 1;
+        }
+        at += __popc(b);
+      }
+    }
+    if (lane == 0) c.lengths[seq] = n;
+  }
+}
+
+// Sequence l.b[i] becomes a fork of l.a[i]: what it held is dropped, full
+// pages are shared, a partly filled tail page is copied.
+__global__ void __launch_bounds__(kPlanThreads) k_fork(KvArgs c, const __grid_constant__ KvList l) {
+  pdl_wait();
+  pdl_trigger();
+  const Work w = work_of(c);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kW = kPlanThreads / 32;
+  const int ps = 1 << c.g.shift;
+  auto add_dropped = [&](int d) {
+    for (int i = warp; i < l.n; i += kW)
+      for (int j = lane; j < c.g.max_pages; j += 32) {
+        const int p = table_page(c, l.b[i], j);
+        if (p >= 0) atomicAdd(c.refs + p, d);
+      }
+  };
+  add_dropped(-1);
+  __syncthreads();
+  // the page each fork has to copy, if any
+  int tail_page = -1, n = 0;
+  if (threadIdx.x < l.n) {
+    n = checked_length(c, l.a[threadIdx.x]);
+    if (n & (ps - 1)) tail_page = table_page(c, l.a[threadIdx.x], n >> c.g.shift);
+  }
+  int total;
+  const int at = block_scan(tail_page >= 0, &total);
+  if (!find_free(c, w, total)) {
+    add_dropped(1);
+    if (threadIdx.x == 0) {
+      *w.copies = 0;
+      kv_status(c, kKvOutOfPages);
+    }
+    return;
+  }
+  __shared__ int s_new[kKvMaxList];
+  if (threadIdx.x < l.n) {
+    int page = -1;
+    if (tail_page >= 0) {
+      page = w.map[at];
+      w.src[at] = tail_page;
+      w.dst[at] = page;
+    }
+    s_new[threadIdx.x] = page;
+  }
+  if (threadIdx.x == 0) *w.copies = total;
+  __syncthreads();
+  for (int i = warp; i < l.n; i += kW) {
+    const int len = checked_length(c, l.a[i]), full = len >> c.g.shift;
+    int* row = c.table + (long long)l.b[i] * c.g.max_pages;
+    for (int j = lane; j < c.g.max_pages; j += 32) {
+      int p = j < full ? table_page(c, l.a[i], j) : -1;
+      if (p >= 0) atomicAdd(c.refs + p, 1);
+      if (j == full && s_new[i] >= 0) {
+        p = s_new[i];
+        c.refs[p] = 1;
+      }
+      row[j] = p;
+    }
+    if (lane == 0) c.lengths[l.b[i]] = len;
+  }
+}
+
+// One block per listed sequence: all its pages (window < 0), or those wholly
+// behind the window and past the sinks, are given back.
+__global__ void __launch_bounds__(256)
+    k_drop(KvArgs c, const __grid_constant__ KvList l, int window, int sinks) {
+  pdl_wait();
+  pdl_trigger();
+  const int seq = l.a[blockIdx.x];
+  int* row = c.table + (long long)seq * c.g.max_pages;
+  const int len = checked_length(c, seq);
+  for (int j = threadIdx.x; j < c.g.max_pages; j += 256) {
+    if (window >= 0 && !kv_page_behind(j, c.g.shift, len, window, sinks)) continue;
+    const int p = table_page(c, seq, j);
+    if (p >= 0) atomicSub(c.refs + p, 1);
+    row[j] = -1;
+  }
+  if (window < 0 && threadIdx.x == 0) c.lengths[seq] = 0;
+}
+
+// Compaction's plan: with L live pages, the k-th live page at or above L moves
+// to the k-th free index below L.
+__global__ void __launch_bounds__(kPlanThreads) k_plan_compact(KvArgs c) {
+  pdl_wait();
+  pdl_trigger();
+  const Work w = work_of(c);
+  int mine = 0;
+  for (int p = threadIdx.x; p < c.g.pages; p += kPlanThreads) mine += __ldcg(c.refs + p) > 0;
+  int live;
+  block_scan(mine, &live);
+  int holes = 0, moved = 0;
+  for (int p0 = 0; p0 < c.g.pages; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int used = p < c.g.pages && __ldcg(c.refs + p) > 0;
+    const int hole = p < live && !used, move = p >= live && used;
+    int n;
+    const int at = block_scan(hole | (move << 16), &n);
+    if (hole) w.dst[holes + (at & 0xffff)] = p;
+    if (move) w.src[moved + (at >> 16)] = p;
+    holes += n & 0xffff;
+    moved += n >> 16;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < moved; i += kPlanThreads) {
+    const int s = __ldcg(w.src + i), d = __ldcg(w.dst + i);
+    w.map[s] = d;
+    c.refs[d] = __ldcg(c.refs + s);
+    c.refs[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *w.copies = moved;
+    w.copies[1] = live;
+  }
+}
+
+// Copies the listed pages, 16 bytes per thread and step, four steps in
+// flight; a page is cut into pieces so that few pages still fill the device.
+// With `remap`, the table entries that name a moved page follow it.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyPiece = kCopyThreads * 4 * 16;
+
+__global__ void __launch_bounds__(kCopyThreads) k_copy_pages(KvArgs c, int remap) {
+  pdl_wait();
+  pdl_trigger();
+  const Work w = work_of(c);
+  const int copies = __ldcg(w.copies);
+  const long long bytes = kv_page_bytes(c.g);
+  const int pieces = (int)((bytes + kCopyPiece - 1) / kCopyPiece);
+  const long long units = (long long)copies * pieces;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int i = (int)(u / pieces);
+    const long long b0 = (u - (long long)i * pieces) * kCopyPiece;
+    const unsigned char* s = c.pool + __ldcg(w.src + i) * bytes + b0;
+    unsigned char* d = c.pool + __ldcg(w.dst + i) * bytes + b0;
+    uint4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long o = (long long)(k * kCopyThreads + threadIdx.x) * 16;
+      if (b0 + o < bytes) x[k] = __ldcg(reinterpret_cast<const uint4*>(s + o));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long o = (long long)(k * kCopyThreads + threadIdx.x) * 16;
+      if (b0 + o < bytes) *reinterpret_cast<uint4*>(d + o) = x[k];
+    }
+  }
+  if (remap && copies > 0) {
+    const int live = __ldcg(w.copies + 1);
+    const long long n = (long long)c.g.seqs * c.g.max_pages;
+    for (long long e = (long long)blockIdx.x * kCopyThreads + threadIdx.x; e < n;
+         e += (long long)gridDim.x * kCopyThreads) {
+      const int p = __ldcg(c.table + e);
+      if (p >= live && p < c.g.pages) c.table[e] = __ldcg(w.map + p);
+    }
+  }
+}
+
+cudaError_t copy_pages(const KvArgs& c, int remap, cudaStream_t stream) {
+  return launch(k_copy_pages, dim3(148 * 8), dim3(kCopyThreads), 0, stream, c, remap);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_resize(const KvArgs& c, const KvList& l, cudaStream_t stream) {
+  if (l.n == 0) return cudaSuccess;
+  const cudaError_t e = launch(k_resize, dim3(1), dim3(kPlanThreads), 0, stream, c, l);
+  return e != cudaSuccess ? e : copy_pages(c, 0, stream);
+}
+cudaError_t launch_kv_fork(const KvArgs& c, const KvList& l, cudaStream_t stream) {
+  if (l.n == 0) return cudaSuccess;
+  const cudaError_t e = launch(k_fork, dim3(1), dim3(kPlanThreads), 0, stream, c, l);
+  return e != cudaSuccess ? e : copy_pages(c, 0, stream);
+}
+cudaError_t launch_kv_drop(const KvArgs& c, const KvList& l, int window, int sinks,
+                           cudaStream_t stream) {
+  if (l.n == 0) return cudaSuccess;
+  return launch(k_drop, dim3((unsigned)l.n), dim3(256), 0, stream, c, l, window, sinks);
+}
+cudaError_t launch_kv_compact(const KvArgs& c, cudaStream_t stream) {
+  const cudaError_t e = launch(k_plan_compact, dim3(1), dim3(kPlanThreads), 0, stream, c);
+  return e != cudaSuccess ? e : copy_pages(c, 1, stream);
+}
+
+}  // namespace qtts

@@ -139,6 +139,16 @@ SIGNATURES = {
     "qtts_last_timings": (C.c_int32, [_P, _F, _F, _SZ]),
     "qtts_last_launch_count": (C.c_int32, [_P, _SZ]),
     "qtts_profile_projection": (C.c_int32, [_P, C.c_int32, C.c_int32, _F, C.POINTER(C.c_double)]),
+    "qtts_kv_sizes": (C.c_int32, [_P, _SZ, _SZ]),
+    "qtts_kv_append": (C.c_int32, [_P, C.c_int32, _P, _P, C.c_size_t, C.c_size_t, _P, C.c_size_t, C.c_size_t, C.c_int32, _P]),
+    "qtts_kv_read": (C.c_int32, [_P, C.c_int32, _P, _P, C.c_size_t, C.c_size_t, _P, C.c_size_t, C.c_size_t, C.c_int32, _P]),
+    "qtts_kv_attend": (C.c_int32, [_P, C.c_int32, _P, _P, C.c_size_t, C.c_size_t, _P, C.c_size_t, C.c_size_t, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_int32, _P]),
+    "qtts_kv_resize": (C.c_int32, [_P, _I32, _I32, C.c_size_t, _P]),
+    "qtts_kv_fork": (C.c_int32, [_P, _I32, _I32, C.c_size_t, _P]),
+    "qtts_kv_free": (C.c_int32, [_P, _I32, C.c_size_t, _P]),
+    "qtts_kv_evict": (C.c_int32, [_P, _I32, C.c_size_t, C.c_int32, C.c_int32, _P]),
+    "qtts_kv_compact": (C.c_int32, [_P, _P]),
+    "qtts_kv_check": (C.c_int32, [_P, _P]),
 }
 
 

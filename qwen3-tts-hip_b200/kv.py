@@ -1,0 +1,272 @@
+"""Paged key / value caches over torch tensors (the qtts_kv_* entry points).
+
+``KvCache`` holds four CUDA tensors (pool, page table, lengths, reference
+counts) and runs the library's kernels on them: ``append`` / ``read`` rows,
+``attend`` with an optional sliding window and first positions that stay
+visible, and ``resize`` / ``fork`` / ``free`` / ``evict`` / ``compact`` pages.
+The pool keeps 16-bit (bf16) or 4-bit rows; the layout of both is stated in
+``include/qtts_b200.h``.
+
+Calls enqueue on torch's current stream of the cache's device, allocate
+nothing but their results, and may be captured into a CUDA graph (lists and
+lengths given from the host are fixed at capture). What only the device can
+tell (too few free pages, a bad index in a device array) is recorded there;
+``check()`` waits for the stream and raises it. Calls on one cache must be
+ordered: one stream, or events between streams.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+from . import engine as _e
+
+F32, BF16 = 0, 1
+HEAD_DIM = 128
+_INT_MAX = 2 ** 31 - 1
+
+
+class _Cache(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("refs", C.c_void_p), ("work", C.c_void_p), ("device", C.c_int32),
+                ("pages", C.c_int32), ("seqs", C.c_int32), ("max_pages", C.c_int32),
+                ("layers", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("bits", C.c_int32)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("seqs", C.c_void_p), ("row_start", C.c_void_p), ("groups", C.c_int32),
+                ("rows", C.c_int32), ("max_rows", C.c_int32), ("max_length", C.c_int32)]
+
+
+def _invalid(message: str):
+    raise _e.InvalidInput(_e.ERR_INVALID_INPUT, message)
+
+
+def _int(v, name: str) -> int:
+    # ctypes would cut a larger value to 32 bits without a word
+    if not -_INT_MAX <= v <= _INT_MAX:
+        _invalid(f"{name} is outside 32 bits: {v}")
+    return v
+
+
+class KvCache:
+    """A paged key / value cache (qtts_kv_cache) over the caller's tensors.
+
+    pool        contiguous, any dtype, at least ``pool_bytes``
+    page_table  int32 [seqs, max_pages], -1 where no page
+    lengths     int32 [seqs]
+    refs        int32 [pages]: table entries that name each page
+
+    ``KvCache.allocate`` makes an empty one.
+    """
+
+    def __init__(self, pool, page_table, lengths, refs, *, layers: int, kv_heads: int,
+                 page_size: int = 32, kv_bits: int = 16):
+        import torch
+
+        self._torch = torch
+        for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1),
+                              ("refs", refs, 1)):
+            if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous():
+                _invalid(f"{name} must be a contiguous int32 tensor of {dims} dimension(s)")
+        for name, t in (("pool", pool), ("page_table", page_table), ("lengths", lengths),
+                        ("refs", refs)):
+            if t.device.type != "cuda" or t.device != pool.device:
+                _invalid(f"{name} must be on the pool's CUDA device")
+        if not pool.is_contiguous():
+            _invalid("pool must be contiguous")
+        if lengths.shape[0] != page_table.shape[0]:
+            _invalid(f"lengths has {lengths.shape[0]} sequences, page_table {page_table.shape[0]}")
+        self.pool, self.page_table, self.lengths, self.refs = pool, page_table, lengths, refs
+        self.layers, self.kv_heads = int(layers), int(kv_heads)
+        self.page_size, self.kv_bits = int(page_size), int(kv_bits)
+        self.device = pool.device
+        self._index = pool.device.index if pool.device.index is not None else 0
+        c = _Cache(pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+                   None, self._index, refs.shape[0], page_table.shape[0], page_table.shape[1],
+                   self.layers, self.kv_heads, self.page_size, self.kv_bits)
+        bytes_, ints = C.c_size_t(), C.c_size_t()
+        L = _e.lib()
+        _e._check(L.qtts_kv_sizes(C.byref(c), C.byref(bytes_), C.byref(ints)))
+        self.pool_bytes = bytes_.value
+        if pool.numel() * pool.element_size() < self.pool_bytes:
+            _invalid(f"pool holds {pool.numel() * pool.element_size()} bytes, "
+                     f"{c.pages} pages need {self.pool_bytes}")
+        self._work = torch.zeros(ints.value, dtype=torch.int32, device=pool.device)
+        # zeroed before any stream may use it
+        torch.cuda.current_stream(pool.device).synchronize()
+        c.work = self._work.data_ptr()
+        self._c, self._ref = c, C.byref(c)
+        self._lib = L
+        self._stream_of = torch._C._cuda_getCurrentRawStream
+        self._home = self._stream_of(self._index)
+
+    @classmethod
+    def allocate(cls, seqs: int, max_length: int, *, layers: int, kv_heads: int,
+                 pages: Optional[int] = None, page_size: int = 32, kv_bits: int = 16,
+                 device: int = 0) -> "KvCache":
+        """An empty cache for ``seqs`` sequences of up to ``max_length``
+        positions; ``pages`` pages in all (default: enough for every one)."""
+        import torch
+
+        for name, v in (("seqs", seqs), ("max_length", max_length), ("page_size", page_size)):
+            if int(v) <= 0:
+                _invalid(f"{name} must be positive, got {v}")
+        width = -(-int(max_length) // int(page_size))
+        pages = int(seqs) * width if pages is None else int(pages)
+        c = _Cache(None, None, None, None, None, int(device), pages, int(seqs), width, int(layers),
+                   int(kv_heads), int(page_size), int(kv_bits))
+        bytes_ = C.c_size_t()
+        _e._check(_e.lib().qtts_kv_sizes(C.byref(c), C.byref(bytes_), None))
+        where = torch.device("cuda", int(device))
+        return cls(torch.empty(bytes_.value, dtype=torch.uint8, device=where),
+                   torch.full((int(seqs), width), -1, dtype=torch.int32, device=where),
+                   torch.zeros(int(seqs), dtype=torch.int32, device=where),
+                   torch.zeros(pages, dtype=torch.int32, device=where),
+                   layers=layers, kv_heads=kv_heads, page_size=page_size, kv_bits=kv_bits)
+
+    # ---- rows
+    def _stream(self) -> int:
+        s = self._stream_of(self._index)
+        if s != self._home:  # memory of another stream's: kept until this one is done with it
+            cur = self._torch.cuda.current_stream(self.device)
+            for t in (self.pool, self.page_table, self.lengths, self.refs, self._work):
+                t.record_stream(cur)
+        return s
+
+    def _dtype(self, t, name: str, heads: Optional[int] = None) -> int:
+        torch = self._torch
+        d = t.dtype
+        code = F32 if d is torch.float32 else BF16 if d is torch.bfloat16 else -1
+        if code < 0:
+            _invalid(f"{name} must be float32 or bfloat16, got {d}")
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+            _invalid(f"{name} must be [rows, heads, {HEAD_DIM}] with a contiguous last dimension, "
+                     f"got shape {tuple(t.shape)} and strides {t.stride()}")
+        if t.stride(0) < 0 or t.stride(1) < 0:
+            _invalid(f"{name} has a negative stride")
+        if heads is not None and t.shape[1] != heads:
+            _invalid(f"{name} has {t.shape[1]} heads, the cache {heads}")
+        if t.device != self.device:
+            _invalid(f"{name} is on {t.device}, the cache on {self.device}")
+        return code
+
+    def _index_array(self, t, name: str) -> int:
+        if t.dtype is not self._torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            _invalid(f"{name} must be a contiguous one-dimensional int32 tensor")
+        if t.device != self.device:
+            _invalid(f"{name} is on {t.device}, the cache on {self.device}")
+        return t.data_ptr()
+
+    def _rows(self, rows: int, seqs, row_start, max_rows: int, max_length: int):
+        if not 0 <= rows <= _INT_MAX:
+            _invalid(f"rows must be between 0 and {_INT_MAX}, got {rows}")
+        groups, starts, named = rows, None, None
+        if row_start is not None:
+            starts = self._index_array(row_start, "row_start")
+            groups = row_start.shape[0] - 1
+            if groups < 0:
+                _invalid("row_start must hold at least one entry")
+        if seqs is not None:
+            named = self._index_array(seqs, "seqs")
+            if seqs.shape[0] != groups:
+                _invalid(f"seqs names {seqs.shape[0]} sequences for {groups} groups of rows")
+        return C.byref(_Rows(named, starts, groups, rows, _int(max_rows, "max_rows"),
+                             _int(max_length, "max_length")))
+
+    def append(self, layer: int, k, v, *, seqs=None, row_start=None, max_rows: int = 0) -> None:
+        """Stores rows ``k``, ``v`` [rows, kv_heads, 128]: group i (one row,
+        or rows ``row_start[i]`` .. ``row_start[i + 1] - 1``) are the last rows
+        of sequence ``seqs[i]`` (default i), whose length counts them already
+        (``resize``)."""
+        dt = self._dtype(k, "k", self.kv_heads)
+        if self._dtype(v, "v", self.kv_heads) != dt or v.shape != k.shape:
+            _invalid("k and v must have the same shape and dtype")
+        rows = self._rows(k.shape[0], seqs, row_start, max_rows, 0)
+        _e._check(self._lib.qtts_kv_append(
+            self._ref, _int(layer, "layer"), rows, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), dt, self._stream()))
+
+    def read(self, layer: int, rows: int, *, dtype=None, seqs=None, row_start=None,
+             max_rows: int = 0):
+        """(k, v) [rows, kv_heads, 128] as the cache holds them, rows grouped
+        as in ``append``; zeros where there is no page, undefined for rows
+        outside every group."""
+        torch = self._torch
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            _invalid(f"dtype must be float32 or bfloat16, got {dtype}")
+        groups = self._rows(rows, seqs, row_start, max_rows, 0)
+        kv = torch.empty((2, rows, self.kv_heads, HEAD_DIM), dtype=dtype, device=self.device)
+        half = rows * self.kv_heads * HEAD_DIM * kv.element_size()
+        at = kv.data_ptr()
+        _e._check(self._lib.qtts_kv_read(
+            self._ref, _int(layer, "layer"), groups, at, self.kv_heads * HEAD_DIM, HEAD_DIM, at + half,
+            self.kv_heads * HEAD_DIM, HEAD_DIM, F32 if dtype is torch.float32 else BF16,
+            self._stream()))
+        return kv[0], kv[1]
+
+    def attend(self, layer: int, q, *, window: int = 0, sinks: int = 0,
+               scale: Optional[float] = None, seqs=None, row_start=None, max_rows: int = 0,
+               max_length: int = 0, out=None):
+        """Attention of rows ``q`` [rows, q_heads, 128] over the cache: the row
+        at position p sees positions c <= p with ``p - c < window`` or
+        ``c < sinks`` (``window`` 0: all). ``scale`` defaults to 128 ** -0.5;
+        ``max_rows`` and ``max_length`` only help the launch's shape. Rows that
+        see nothing give zeros; rows outside every group are left as they are
+        (undefined when ``out`` is not given)."""
+        dt = self._dtype(q, "q")
+        if out is None:
+            out = self._torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        elif self._dtype(out, "out") != dt or out.shape != q.shape:
+            _invalid("out must have q's shape and dtype")
+        rows = self._rows(q.shape[0], seqs, row_start, max_rows, max_length)
+        _e._check(self._lib.qtts_kv_attend(
+            self._ref, _int(layer, "layer"), rows, q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1), dt, q.shape[1],
+            HEAD_DIM ** -0.5 if scale is None else scale, _int(window, "window"),
+            _int(sinks, "sinks"), self._stream()))
+        return out
+
+    # ---- pages
+    def _list(self, v: Sequence[int]):
+        try:
+            if len(v) and not (-_INT_MAX <= min(v) and max(v) <= _INT_MAX):
+                _invalid("an entry of the list is outside 32 bits")
+            return (C.c_int32 * len(v))(*v)
+        except TypeError:
+            _invalid("sequence lists must hold integers")
+
+    def resize(self, seqs: Sequence[int], lengths: Sequence[int]) -> None:
+        """Gives each sequence its new length (pages taken or given back)."""
+        if len(seqs) != len(lengths):
+            _invalid("one length per sequence")
+        _e._check(self._lib.qtts_kv_resize(self._ref, self._list(seqs), self._list(lengths),
+                                           len(seqs), self._stream()))
+
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Makes each ``dst`` a copy of its ``src``, sharing full pages."""
+        if len(src) != len(dst):
+            _invalid("one destination per source")
+        _e._check(self._lib.qtts_kv_fork(self._ref, self._list(src), self._list(dst), len(src),
+                                         self._stream()))
+
+    def free(self, seqs: Sequence[int]) -> None:
+        """Empties the sequences."""
+        _e._check(self._lib.qtts_kv_free(self._ref, self._list(seqs), len(seqs), self._stream()))
+
+    def evict(self, seqs: Sequence[int], window: int, sinks: int = 0) -> None:
+        """Gives back the pages that (window, sinks) hides from every row at
+        or after the newest position."""
+        _e._check(self._lib.qtts_kv_evict(self._ref, self._list(seqs), len(seqs),
+                                          _int(window, "window"), _int(sinks, "sinks"),
+                                          self._stream()))
+
+    def compact(self) -> None:
+        """Moves the pages in use to the lowest indices."""
+        _e._check(self._lib.qtts_kv_compact(self._ref, self._stream()))
+
+    def check(self) -> None:
+        """Waits for the stream and raises what the device recorded."""
+        _e._check(self._lib.qtts_kv_check(self._ref, self._stream()))

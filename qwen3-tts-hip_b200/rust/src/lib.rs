@@ -131,6 +131,39 @@ pub mod ffi {
         pub samples_per_frame: u32,
     }
 
+    pub const QTTS_F32: i32 = 0;
+    pub const QTTS_BF16: i32 = 1;
+
+    /// Every pointer is device memory of `device`.
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct qtts_kv_cache {
+        pub pool: *mut (),
+        pub page_table: *mut i32,
+        pub lengths: *mut i32,
+        pub refs: *mut i32,
+        pub work: *mut i32,
+        pub device: i32,
+        pub pages: i32,
+        pub seqs: i32,
+        pub max_pages: i32,
+        pub layers: i32,
+        pub kv_heads: i32,
+        pub page_size: i32,
+        pub bits: i32,
+    }
+
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct qtts_kv_rows {
+        pub seqs: *const i32,
+        pub row_start: *const i32,
+        pub groups: i32,
+        pub rows: i32,
+        pub max_rows: i32,
+        pub max_length: i32,
+    }
+
     #[link(name = "qtts_b200")]
     extern "C" {
         pub fn qtts_last_error() -> *const c_char;
@@ -236,6 +269,28 @@ pub mod ffi {
         pub fn qtts_profile_projection(engine: *mut qtts_engine, which: i32, launches: i32,
                                        ms_per_launch: *mut f32,
                                        bytes_per_launch: *mut f64) -> i32;
+        pub fn qtts_kv_sizes(cache: *const qtts_kv_cache, pool_bytes: *mut usize,
+                             work_ints: *mut usize) -> i32;
+        pub fn qtts_kv_append(cache: *const qtts_kv_cache, layer: i32, rows: *const qtts_kv_rows,
+                              k: *const (), k_row: usize, k_head: usize, v: *const (),
+                              v_row: usize, v_head: usize, dtype: i32, stream: *mut ()) -> i32;
+        pub fn qtts_kv_read(cache: *const qtts_kv_cache, layer: i32, rows: *const qtts_kv_rows,
+                            k: *mut (), k_row: usize, k_head: usize, v: *mut (), v_row: usize,
+                            v_head: usize, dtype: i32, stream: *mut ()) -> i32;
+        pub fn qtts_kv_attend(cache: *const qtts_kv_cache, layer: i32, rows: *const qtts_kv_rows,
+                              q: *const (), q_row: usize, q_head: usize, out: *mut (),
+                              out_row: usize, out_head: usize, dtype: i32, q_heads: i32,
+                              scale: f32, window: i32, sinks: i32, stream: *mut ()) -> i32;
+        pub fn qtts_kv_resize(cache: *const qtts_kv_cache, seqs: *const i32, lengths: *const i32,
+                              n: usize, stream: *mut ()) -> i32;
+        pub fn qtts_kv_fork(cache: *const qtts_kv_cache, src: *const i32, dst: *const i32,
+                            n: usize, stream: *mut ()) -> i32;
+        pub fn qtts_kv_free(cache: *const qtts_kv_cache, seqs: *const i32, n: usize,
+                            stream: *mut ()) -> i32;
+        pub fn qtts_kv_evict(cache: *const qtts_kv_cache, seqs: *const i32, n: usize,
+                             window: i32, sinks: i32, stream: *mut ()) -> i32;
+        pub fn qtts_kv_compact(cache: *const qtts_kv_cache, stream: *mut ()) -> i32;
+        pub fn qtts_kv_check(cache: *const qtts_kv_cache, stream: *mut ()) -> i32;
     }
 }
 
