@@ -55,6 +55,9 @@ cudaError_t launch_kv_append(const KvArgs& c, const KvRows& r, int layer, const 
                              const KvTensor& v, int type, cudaStream_t stream);
 cudaError_t launch_kv_read(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                            const KvTensor& v, int type, cudaStream_t stream);
+// One CTA or cluster per row (and kv head).
+cudaError_t launch_kv_step(const KvArgs& c, const KvRows& r, const KvAttend& a,
+                           cudaStream_t stream);
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream);
 

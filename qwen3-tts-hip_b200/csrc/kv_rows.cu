@@ -156,6 +156,7 @@ cudaError_t launch_kv_read(const KvArgs& c, const KvRows& r, int layer, const Kv
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream) {
   if (r.rows == 0) return cudaSuccess;
+  if (r.max_rows <= 8) return launch_kv_step(c, r, a, stream);
   return launch(k_kv_attend_simple, dim3((unsigned)a.q_heads, (unsigned)((r.rows + 3) / 4)),
                 dim3(128), 0, stream, c, r, a);
 }

@@ -1,0 +1,516 @@
+// Attention of single rows over a paged key / value cache (decode steps and
+// chunks of a few rows), bound by reading the cache.
+//
+// One CTA (or a cluster of them, each with a share of the positions) serves
+// one row's query heads of one kv head, at most four. A warp takes tiles of 16
+// positions straight from global memory into the registers of the matrix
+// instruction, with no shared memory between:
+//   S^T[16 positions][8] = K[16][128] * Q^T      (K the 16-row operand)
+//   O^T[128 dims][8]    += V^T[128][16] * P^T    (V^T the 16-row operand)
+// The order of the summed index is free, so each lane's 16-byte loads are
+// operand fragments as they are (K) or after one byte permute per pair (V).
+// The 8 columns are (head t, part 0 or 1) = column 2 t + part: what a bf16
+// operand cannot hold of a query or a weight goes into its second part (and,
+// for fp32 rows, a third one through a second instruction into the same
+// accumulators), so products keep 16 bits for bf16 rows and 24 for fp32 ones.
+// Column pairs 2 t, 2 t + 1 of an accumulator sit in one lane: summing the
+// parts costs one addition.
+//
+// 4-bit rows: codes become bf16 integers (exact) by bit operations. K: each
+// group of 32 dims accumulates apart and its scale multiplies the fp32 sum; V:
+// the scale multiplies the fp32 weight before it is split into parts.
+//
+// Statistics, scores and sums are fp32. Warps merge through shared memory,
+// CTAs of a cluster through distributed shared memory, both in a fixed order.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "common.cuh"
+#include "kv.cuh"
+#include "sm100.cuh"
+
+namespace qtts {
+namespace {
+
+constexpr int kStepWarps = 8;
+constexpr int kStepThreads = kStepWarps * 32;
+constexpr int kStepHeads = 4;   // query heads of one CTA
+constexpr int kTile = 16;       // positions of one matrix instruction; a page is a multiple
+constexpr int kMaxCluster = 16;
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      " {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Nibbles i and i + 4 (of the two 16-bit halves: one each) of w as bf16
+// integers n = code - 8: 128 + code is a bf16 with the code in its low bits.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
+  const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
+                                   __nv_bfloat162(__float2bfloat16(136.f), __float2bfloat16(136.f)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// What one lane (g = lane / 4, t = lane % 4) loads of a tile.
+template <int BITS>
+struct Tile;
+template <>
+struct Tile<16> {
+  uint4 k[2][4];  // rows g, g + 8; dims 32 j + 8 t ..
+  uint4 v[4][2];  // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9; dims 8 g .., 64 + 8 g ..
+};
+template <>
+struct Tile<4> {
+  uint4 k[2];     // rows g, g + 8: word j = dims 32 j + 8 t ..
+  uint2 ks[2];    // their four scales
+  uint4 v[4];     // positions as above: word j holds dims 32 j + 8 (g / 2) ..
+  uint2 vs[4];
+};
+
+__device__ __forceinline__ int v_pos(int t, int i) { return 2 * t + (i & 1) + 8 * (i >> 1); }
+
+template <int BITS>
+__device__ __forceinline__ void load_tile(Tile<BITS>& x, const unsigned char* kt,
+                                          const unsigned char* vt, int row0, int shift) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if constexpr (BITS == 16) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x.k[r][j] = __ldcg(reinterpret_cast<const uint4*>(kt + (row0 + g + 8 * r) * 256) + 4 * j + t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        x.v[i][h] = __ldcg(reinterpret_cast<const uint4*>(vt + (row0 + v_pos(t, i)) * 256) + 8 * h + g);
+  } else {
+    const unsigned char* ks = kt + (kKvCodeBytes << shift);
+    const unsigned char* vs = vt + (kKvCodeBytes << shift);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      x.k[r] = __ldcg(reinterpret_cast<const uint4*>(kt + (row0 + g + 8 * r) * 64) + t);
+      x.ks[r] = __ldcg(reinterpret_cast<const uint2*>(ks) + row0 + g + 8 * r);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x.v[i] = __ldcg(reinterpret_cast<const uint4*>(vt + (row0 + v_pos(t, i)) * 64) + (g >> 1));
+      x.vs[i] = __ldcg(reinterpret_cast<const uint2*>(vs) + row0 + v_pos(t, i));
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+__device__ __forceinline__ float scale_of(const uint2& s, int j) {
+  const uint32_t w = j < 2 ? s.x : s.y;
+  return j & 1 ? bf16hi(w) : bf16lo(w);
+}
+
+// Query fragments: column g = (head g / 2, part g % 2), dims as a lane of K
+// holds them. [..][1] (fp32 rows): the third part, in the even columns.
+template <bool F32>
+struct Query {
+  uint32_t b[8][F32 ? 4 : 2];
+};
+
+template <int BITS, bool F32>
+__device__ __forceinline__ void load_query(Query<F32>& q, const void* p, long long off, bool in) {
+  const int lane = threadIdx.x & 31, t = lane & 3, part = (lane >> 2) & 1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float x[8];
+    const float4 a = in ? kv_load4(p, off + 32 * j + 8 * t, F32 ? KV_F32 : KV_BF16)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 b = in ? kv_load4(p, off + 32 * j + 8 * t + 4, F32 ? KV_F32 : KV_BF16)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      // pairs of the summed index, in the order of the K fragments
+      constexpr int pair16[4][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}};
+      constexpr int pair4[4][2] = {{0, 4}, {1, 5}, {2, 6}, {3, 7}};
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int* d = BITS == 16 ? pair16[2 * s + w] : pair4[2 * s + w];
+        const float lo = x[d[0]], hi = x[d[1]];
+        if constexpr (!F32) {
+          q.b[2 * j + s][w] = part ? 0u : pack_bf16(lo, hi);
+        } else {
+          const float l1 = bf16_round(lo), h1 = bf16_round(hi);
+          const float l2 = bf16_round(lo - l1), h2 = bf16_round(hi - h1);
+          q.b[2 * j + s][w] = part ? pack_bf16(l2, h2) : pack_bf16(l1, h1);
+          q.b[2 * j + s][2 + w] = part ? 0u : pack_bf16(lo - l1 - l2, hi - h1 - h2);
+        }
+      }
+    }
+  }
+}
+
+// Splits two weights into this column's part; *third: the even columns' last.
+template <bool F32>
+__device__ __forceinline__ uint32_t weight_parts(float a, float b, int part, uint32_t* third) {
+  const uint32_t hi = pack_bf16(a, b);
+  const float ra = a - bf16lo(hi), rb = b - bf16hi(hi);
+  const uint32_t mid = pack_bf16(ra, rb);
+  if constexpr (F32) *third = part ? 0u : pack_bf16(ra - bf16lo(mid), rb - bf16hi(mid));
+  return part ? mid : hi;
+}
+
+template <int BITS, bool F32>
+struct Warp {
+  float m, l;       // running maximum (head t) and this lane's share of the sum
+  float o[8][4];    // O^T: [m-tile][.]
+
+  // Scores of positions row g (s0) and g + 8 (s1) for head t.
+  __device__ __forceinline__ void scores(const Tile<BITS>& x, const Query<F32>& q, float& s0,
+                                         float& s1) {
+    if constexpr (BITS == 16) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t a[4] = {word(x.k[0][j], 2 * s), word(x.k[1][j], 2 * s),
+                                 word(x.k[0][j], 2 * s + 1), word(x.k[1][j], 2 * s + 1)};
+          mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
+          if constexpr (F32) mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
+        }
+      s0 = c[0] + c[1];
+      s1 = c[2] + c[3];
+    } else {
+      s0 = s1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t w0 = word(x.k[0], j), w1 = word(x.k[1], j);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t a[4] = {nibbles(w0, 2 * s), nibbles(w1, 2 * s), nibbles(w0, 2 * s + 1),
+                                 nibbles(w1, 2 * s + 1)};
+          mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
+          if constexpr (F32) mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
+        }
+        s0 = fmaf(scale_of(x.ks[0], j), c[0] + c[1], s0);
+        s1 = fmaf(scale_of(x.ks[1], j), c[2] + c[3], s1);
+      }
+    }
+  }
+
+  // O^T += V^T P^T; w[i]: this column's weights at v_pos(t, i).
+  __device__ __forceinline__ void values(const Tile<BITS>& x, const float (&w)[4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, part = g & 1;
+    if constexpr (BITS == 16) {
+      uint32_t t0 = 0u, t1 = 0u;
+      const uint32_t b0 = weight_parts<F32>(w[0], w[1], part, &t0);
+      const uint32_t b1 = weight_parts<F32>(w[2], w[3], part, &t1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned sel = i & 1 ? 0x7632u : 0x5410u;
+        uint32_t a[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          a[h] = __byte_perm(word(x.v[0][h], i >> 1), word(x.v[1][h], i >> 1), sel);
+          a[2 + h] = __byte_perm(word(x.v[2][h], i >> 1), word(x.v[3][h], i >> 1), sel);
+        }
+        mma16816(o[i], a, b0, b1);
+        if constexpr (F32) mma16816(o[i], a, t0, t1);
+      }
+    } else {
+      const unsigned sel = part ? 0x7632u : 0x5410u;  // g odd: the word's upper four dims
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t t0 = 0u, t1 = 0u;
+        const uint32_t b0 = weight_parts<F32>(w[0] * scale_of(x.vs[0], j),
+                                              w[1] * scale_of(x.vs[1], j), part, &t0);
+        const uint32_t b1 = weight_parts<F32>(w[2] * scale_of(x.vs[2], j),
+                                              w[3] * scale_of(x.vs[3], j), part, &t1);
+        const uint32_t y0 = __byte_perm(word(x.v[0], j), word(x.v[1], j), sel);
+        const uint32_t y1 = __byte_perm(word(x.v[2], j), word(x.v[3], j), sel);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t a[4] = {nibbles(y0, 2 * i), nibbles(y0, 2 * i + 1), nibbles(y1, 2 * i),
+                                 nibbles(y1, 2 * i + 1)};
+          mma16816(o[2 * j + i], a, b0, b1);
+          if constexpr (F32) mma16816(o[2 * j + i], a, t0, t1);
+        }
+      }
+    }
+  }
+
+  // The output dim of accumulator o[i][2 * h] (+ o[i][2 * h + 1]: parts).
+  __device__ static __forceinline__ int dim_of(int g, int i, int h) {
+    return BITS == 16 ? 64 * h + 8 * g + i : 32 * (i >> 1) + 4 * g + 2 * (i & 1) + h;
+  }
+};
+
+// Partial result of one CTA (or warp): per head its maximum, sum, and sum of
+// weighted values.
+struct Partial {
+  float m[kStepHeads], l[kStepHeads];
+  float o[kStepHeads][kKvDim];
+};
+
+template <int BITS, bool F32>
+__global__ void __launch_bounds__(kStepThreads, 1)
+    k_kv_step(KvArgs c, KvRows r, KvAttend a, int chunks) {
+  constexpr int TILES = BITS == 16 ? 1 : 2;  // tiles in flight per step: registers
+  __shared__ Partial s_warp[kStepWarps];
+  __shared__ Partial s_cta;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int ctas = (int)cluster_size_x(), rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
+  const int head = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+  const int group = a.q_heads / c.g.kv_heads;
+  const int heads = min(kStepHeads, group - chunk * kStepHeads);
+  const int qh0 = head * group + chunk * kStepHeads;
+  const KvPlace at = kv_place(c, r, row, false);
+  // uniform over the cluster: the decision depends on the row alone
+  if (at.group < 0 || (a.halt && __ldcg(a.halt + (long long)at.group * a.halt_stride))) return;
+  Query<F32> q;
+  load_query<BITS, F32>(q, a.q.p, (long long)row * a.q.row + (long long)(qh0 + (g >> 1)) * a.q.head,
+                        (g >> 1) < heads);
+  // visible tiles: [0, ns) and [ws, pos / 16]
+  const KvSpan sp = kv_span(at.ok ? at.pos : 0, a.window, a.sinks);
+  const int ns = (sp.sink_end + kTile - 1) / kTile;
+  const int ws = max(sp.first / kTile, ns);
+  const int total = at.ok ? ns + at.pos / kTile - ws + 1 : 0;
+  Warp<BITS, F32> acc;
+  acc.m = -INFINITY;
+  acc.l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc.o[i][k] = 0.f;
+
+  const int stride = ctas * kStepWarps, wg = rank * kStepWarps + warp;
+  const int steps = total > wg * TILES ? (total - wg * TILES + stride * TILES - 1) / (stride * TILES) : 0;
+  auto tile_of = [&](int it, int u) {
+    const int i = (it * stride + wg) * TILES + u;
+    return i >= total ? -1 : i < ns ? i : i - ns + ws;
+  };
+  const long long tile_bytes = kv_tile_bytes(c.g), page_bytes = kv_page_bytes(c.g);
+  const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
+  const unsigned char* vbase = kbase + tile_bytes * c.g.kv_heads;
+  int pages[TILES];  // lane i: the page of tile tile_of(32 * block + i, u)
+  Tile<BITS> cur[TILES], nxt[TILES];
+  auto fetch = [&](int it, Tile<BITS> (&x)[TILES]) {
+    if ((it & 31) == 0) {
+#pragma unroll
+      for (int u = 0; u < TILES; ++u) {
+        const int tl = tile_of(it + lane, u);
+        pages[u] = tl >= 0 ? kv_page(c, at.seq, (tl * kTile) >> c.g.shift) : -1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) {
+      // a tile that is not there is read from page 0 and masked
+      const int page = max(0, __shfl_sync(0xffffffffu, pages[u], it & 31));
+      const int tl = max(0, tile_of(it, u));
+      load_tile<BITS>(x[u], kbase + page * page_bytes, vbase + page * page_bytes,
+                      (tl * kTile) & ((1 << c.g.shift) - 1), c.g.shift);
+    }
+  };
+  auto have = [&](int it, int u) {  // before the pages of the next block are fetched
+    return __shfl_sync(0xffffffffu, pages[u], it & 31) >= 0;
+  };
+  if (steps) fetch(0, cur);
+  for (int it = 0; it < steps; ++it) {
+    bool there[TILES];
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) there[u] = have(it, u);
+    if (it + 1 < steps) fetch(it + 1, nxt);
+    float s[TILES][2];
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) {
+      acc.scores(cur[u], q, s[u][0], s[u][1]);
+      s[u][0] *= a.scale;
+      s[u][1] *= a.scale;
+      const int p0 = tile_of(it, u) * kTile;
+      const bool full = there[u] && p0 + kTile - 1 <= at.pos &&
+                        (a.window == 0 || p0 > at.pos - a.window || p0 + kTile <= a.sinks);
+      if (!full) {
+        auto vis = [&](int p) { return there[u] && kv_sees(at.pos, p, a.window, a.sinks); };
+        if (!vis(p0 + g)) s[u][0] = -INFINITY;
+        if (!vis(p0 + g + 8)) s[u][1] = -INFINITY;
+        // what a masked row holds must not meet its zero weight: it may be NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!vis(p0 + v_pos(t, i))) {
+            if constexpr (BITS == 16)
+              cur[u].v[i][0] = cur[u].v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            else
+              cur[u].vs[i] = make_uint2(0u, 0u);
+          }
+      }
+      top = fmaxf(top, fmaxf(s[u][0], s[u][1]));
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (__any_sync(0xffffffffu, top > acc.m)) {
+      const float m = fmaxf(acc.m, top);
+      // no finite score yet: nothing to rescale (and -inf - -inf is not a number)
+      const float f = m == -INFINITY ? 1.f : exp2f((acc.m - m) * 1.4426950408889634f);
+      acc.m = m;
+      acc.l *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc.o[i][k] *= f;
+    }
+    const float ref = acc.m == -INFINITY ? 0.f : acc.m;
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) {
+      const float w0 = exp2f((s[u][0] - ref) * 1.4426950408889634f);
+      const float w1 = exp2f((s[u][1] - ref) * 1.4426950408889634f);
+      acc.l += w0 + w1;
+      // weights of (positions 2 t, 2 t + 1 and + 8; head g / 2): from the lanes
+      // that hold them as (position g', head t')
+      float w[4];
+      const int src = 8 * t + (g >> 1);
+      w[0] = __shfl_sync(0xffffffffu, w0, src);
+      w[1] = __shfl_sync(0xffffffffu, w0, src + 4);
+      w[2] = __shfl_sync(0xffffffffu, w1, src);
+      w[3] = __shfl_sync(0xffffffffu, w1, src + 4);
+      acc.values(cur[u], w);
+    }
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) cur[u] = nxt[u];
+  }
+
+  // warp -> CTA
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) acc.l += __shfl_xor_sync(0xffffffffu, acc.l, o);
+  if (g == 0) {
+    s_warp[warp].m[t] = acc.m;
+    s_warp[warp].l[t] = acc.l;
+  }
+  if (t < heads)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        s_warp[warp].o[t][acc.dim_of(g, i, h)] = acc.o[i][2 * h] + acc.o[i][2 * h + 1];
+  __syncthreads();
+  // the maximum over `n` partials, then the weighted sums; a partial that saw
+  // nothing has m = -inf and weight 0
+  auto out_at = [&](int h, int d) {
+    return (long long)row * a.out.row + (long long)(qh0 + h) * a.out.head + d;
+  };
+  auto put = [&](int h, int d, float v) {
+    if constexpr (F32)
+      static_cast<float*>(a.out.p)[out_at(h, d)] = v;
+    else
+      static_cast<__nv_bfloat16*>(a.out.p)[out_at(h, d)] = __float2bfloat16_rn(v);
+  };
+  for (int e = threadIdx.x; e < heads * kKvDim; e += kStepThreads) {
+    const int h = e / kKvDim, d = e % kKvDim;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) m = fmaxf(m, s_warp[w].m[h]);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float f = exp2f((s_warp[w].m[h] - ref) * 1.4426950408889634f);
+      l = fmaf(f, s_warp[w].l[h], l);
+      o = fmaf(f, s_warp[w].o[h][d], o);
+    }
+    if (ctas == 1) {
+      put(h, d, l == 0.f ? 0.f : o / l);
+    } else {
+      s_cta.o[h][d] = o;
+      if (d == 0) {
+        s_cta.m[h] = m;
+        s_cta.l[h] = l;
+      }
+    }
+  }
+  if (ctas == 1) return;
+  cluster_arrive();
+  cluster_wait();
+  for (int e = rank * kStepThreads + threadIdx.x; e < heads * kKvDim; e += ctas * kStepThreads) {
+    const int h = e / kKvDim, d = e % kKvDim;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int k = 0; k < ctas; ++k) m = fmaxf(m, ld_cluster_f32(cluster_map(&s_cta.m[h], k)));
+    const float ref = m == -INFINITY ? 0.f : m;
+    for (int k = 0; k < ctas; ++k) {
+      const float f = exp2f((ld_cluster_f32(cluster_map(&s_cta.m[h], k)) - ref) * 1.4426950408889634f);
+      l = fmaf(f, ld_cluster_f32(cluster_map(&s_cta.l[h], k)), l);
+      o = fmaf(f, ld_cluster_f32(cluster_map(&s_cta.o[h][d], k)), o);
+    }
+    put(h, d, l == 0.f ? 0.f : o / l);
+  }
+  // no CTA leaves while another may still read its shared memory
+  cluster_arrive();
+  cluster_wait();
+}
+
+template <int BITS, bool F32>
+cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream_t stream) {
+  constexpr int TILES = BITS == 16 ? 1 : 2;
+  auto kernel = k_kv_step<BITS, F32>;
+  // clusters of 16 are past the portable size: asked for once per device
+  static std::mutex mu;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!ready[dev]) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      ready[dev] = true;
+    }
+  }
+  const int group = a.q_heads / c.g.kv_heads;
+  const int chunks = (group + kStepHeads - 1) / kStepHeads;
+  // Split a row's positions over a cluster until every SM has a CTA, as long
+  // as every warp still has a step of its own.
+  const long long units = (long long)r.rows * c.g.kv_heads * chunks;
+  long long longest = kv_capacity(c.g);
+  if (r.max_length) longest = std::min<long long>(longest, r.max_length);
+  if (a.window) longest = std::min<long long>(longest, (long long)a.window + a.sinks + 2 * kTile);
+  const long long per_cta = (long long)kStepWarps * TILES * kTile;
+  int ctas = 1;
+  while (ctas < kMaxCluster && units * ctas < 148 && longest > per_cta * ctas) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(r.rows * (long long)ctas), (unsigned)(c.g.kv_heads * chunks));
+  cfg.blockDim = dim3(kStepThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, c, r, a, chunks);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_step(const KvArgs& c, const KvRows& r, const KvAttend& a,
+                           cudaStream_t stream) {
+  if (c.g.bits == 16)
+    return a.type == KV_F32 ? step<16, true>(c, r, a, stream) : step<16, false>(c, r, a, stream);
+  return a.type == KV_F32 ? step<4, true>(c, r, a, stream) : step<4, false>(c, r, a, stream);
+}
+
+}  // namespace qtts
