@@ -161,4 +161,64 @@ __device__ __forceinline__ unsigned kv_quantise4(float4 x, float* scale) {
          (kv_code_of(x.w, s) << 12);
 }
 
+// One (row, q head) by one warp, position by position, eight at a time: a
+// running maximum and sum over the visible positions only. The form for rows
+// whose tile holds values that the matrix instructions cannot take (NaN or
+// infinity in a place that some rows of the tile see and others do not; 4-bit
+// scales outside what fp16 holds).
+constexpr int kKvBatch = 8;
+
+__device__ __forceinline__ void kv_attend_row(const KvArgs& c, const KvAttend& a, int seq, int pos,
+                                              int row, int qh) {
+  const int lane = threadIdx.x & 31;
+  const int head = qh / (a.q_heads / c.g.kv_heads);
+  const float4 q =
+      kv_load4(a.q.p, (long long)row * a.q.row + (long long)qh * a.q.head + 4 * lane, a.type);
+  const KvSpan sp = kv_span(pos, a.window, a.sinks);
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int part = 0; part < 2; ++part) {
+    const int begin = part ? sp.first : 0, end = part ? pos + 1 : sp.sink_end;
+    for (int p0 = begin; p0 < end; p0 += kKvBatch) {
+      float4 kf[kKvBatch], vf[kKvBatch];
+      float d[kKvBatch];
+      bool in[kKvBatch];
+#pragma unroll
+      for (int i = 0; i < kKvBatch; ++i) {
+        const int p = p0 + i;
+        const int page = p < end ? kv_page(c, seq, p >> c.g.shift) : -1;
+        in[i] = page >= 0;
+        kf[i] = vf[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in[i]) {
+          kf[i] = kv_cached4(c, page, a.layer, 0, head, p & ((1 << c.g.shift) - 1), lane);
+          vf[i] = kv_cached4(c, page, a.layer, 1, head, p & ((1 << c.g.shift) - 1), lane);
+        }
+        d[i] = q.x * kf[i].x + q.y * kf[i].y + q.z * kf[i].z + q.w * kf[i].w;
+      }
+      float mb = m;
+#pragma unroll
+      for (int i = 0; i < kKvBatch; ++i) {
+        d[i] = in[i] ? warp_sum(d[i]) * a.scale : -INFINITY;
+        mb = fmaxf(mb, d[i]);
+      }
+      const float ref = mb == -INFINITY ? 0.f : mb;
+      const float corr = expf(m - ref);
+      l *= corr;
+      acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
+#pragma unroll
+      for (int i = 0; i < kKvBatch; ++i) {
+        if (!in[i]) continue;
+        const float e = expf(d[i] - ref);
+        l += e;
+        acc.x = fmaf(e, vf[i].x, acc.x); acc.y = fmaf(e, vf[i].y, acc.y);
+        acc.z = fmaf(e, vf[i].z, acc.z); acc.w = fmaf(e, vf[i].w, acc.w);
+      }
+      m = mb;
+    }
+  }
+  const float il = l == 0.f ? 0.f : 1.0f / l;
+  kv_store4(a.out.p, (long long)row * a.out.row + (long long)qh * a.out.head + 4 * lane, a.type,
+            make_float4(acc.x * il, acc.y * il, acc.z * il, acc.w * il));
+}
+
 }  // namespace qtts

@@ -12,6 +12,7 @@ namespace qtts {
 // Bits of the status word (work[0]).
 constexpr int kKvOutOfPages = 1;  // a resize or fork found too few free pages and changed nothing
 constexpr int kKvBadIndex = 2;    // a page, sequence, length or row count out of range was skipped
+constexpr int kKvTimeout = 4;     // a wait inside a kernel ran out (its bound is two seconds)
 
 constexpr int kKvMaxList = 1024;  // sequences of one page-management call
 
@@ -58,6 +59,9 @@ cudaError_t launch_kv_read(const KvArgs& c, const KvRows& r, int layer, const Kv
 // One CTA or cluster per row (and kv head).
 cudaError_t launch_kv_step(const KvArgs& c, const KvRows& r, const KvAttend& a,
                            cudaStream_t stream);
+// Tiles of rows on the tensor cores.
+cudaError_t launch_kv_tiles(const KvArgs& c, const KvRows& r, const KvAttend& a,
+                            cudaStream_t stream);
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream);
 

@@ -285,6 +285,8 @@ int32_t qtts_kv_check(const qtts_kv_cache* cache, void* stream) {
     QCK(cudaStreamSynchronize(stream_of(stream)));
     if (!status) return;
     QCK(cudaMemsetAsync(c.work, 0, sizeof status, stream_of(stream)));
+    if (status & qtts::kKvTimeout)
+      qtts::fail(QTTS_ERR_DEVICE_STATE, "a bounded device wait of the attention pipeline ran out");
     if (status & qtts::kKvBadIndex)
       qtts::fail(QTTS_ERR_DEVICE_STATE,
                  "a sequence, length, row or page of the cache was out of range and was skipped");

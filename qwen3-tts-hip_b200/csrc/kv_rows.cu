@@ -1,5 +1,4 @@
-// Storing rows into a paged key / value cache, loading them back, and the
-// simple form of attention over it.
+// Storing rows into a paged key / value cache and loading them back.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -67,72 +66,6 @@ __global__ void __launch_bounds__(kRowThreads)
   if ((lane & 7) == 0) *sc = __float2bfloat16_rn(s);
 }
 
-// Attention, one warp per (row, q head): a running maximum and sum over the
-// visible positions, eight at a time.
-constexpr int kSimpleBatch = 8;
-
-__global__ void __launch_bounds__(128) k_kv_attend_simple(KvArgs c, KvRows r, KvAttend a) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int qh = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (row >= r.rows) return;
-  const KvPlace at = kv_place(c, r, row, false);
-  if (at.group < 0 || (a.halt && __ldcg(a.halt + (long long)at.group * a.halt_stride))) return;
-  const long long oo = (long long)row * a.out.row + (long long)qh * a.out.head + 4 * lane;
-  if (!at.ok) {
-    kv_store4(a.out.p, oo, a.type, make_float4(0.f, 0.f, 0.f, 0.f));
-    return;
-  }
-  const int head = qh / (a.q_heads / c.g.kv_heads);
-  const float4 q = kv_load4(a.q.p, (long long)row * a.q.row + (long long)qh * a.q.head + 4 * lane, a.type);
-  const KvSpan sp = kv_span(at.pos, a.window, a.sinks);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto run = [&](int begin, int end) {
-    for (int p0 = begin; p0 < end; p0 += kSimpleBatch) {
-      float4 kf[kSimpleBatch], vf[kSimpleBatch];
-      float d[kSimpleBatch];
-      bool in[kSimpleBatch];
-#pragma unroll
-      for (int i = 0; i < kSimpleBatch; ++i) {
-        const int p = p0 + i;
-        const int page = p < end ? kv_page(c, at.seq, p >> c.g.shift) : -1;
-        in[i] = page >= 0;
-        kf[i] = vf[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in[i]) {
-          kf[i] = kv_cached4(c, page, a.layer, 0, head, p & ((1 << c.g.shift) - 1), lane);
-          vf[i] = kv_cached4(c, page, a.layer, 1, head, p & ((1 << c.g.shift) - 1), lane);
-        }
-        d[i] = q.x * kf[i].x + q.y * kf[i].y + q.z * kf[i].z + q.w * kf[i].w;
-      }
-      float mb = m;
-#pragma unroll
-      for (int i = 0; i < kSimpleBatch; ++i) {
-        d[i] = in[i] ? warp_sum(d[i]) * a.scale : -INFINITY;
-        mb = fmaxf(mb, d[i]);
-      }
-      const float ref = mb == -INFINITY ? 0.f : mb;
-      const float corr = expf(m - ref);
-      l *= corr;
-      acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
-#pragma unroll
-      for (int i = 0; i < kSimpleBatch; ++i) {
-        if (!in[i]) continue;
-        const float e = expf(d[i] - ref);
-        l += e;
-        acc.x = fmaf(e, vf[i].x, acc.x); acc.y = fmaf(e, vf[i].y, acc.y);
-        acc.z = fmaf(e, vf[i].z, acc.z); acc.w = fmaf(e, vf[i].w, acc.w);
-      }
-      m = mb;
-    }
-  };
-  run(0, sp.sink_end);
-  run(sp.first, at.pos + 1);
-  const float il = l == 0.f ? 0.f : 1.0f / l;
-  kv_store4(a.out.p, oo, a.type, make_float4(acc.x * il, acc.y * il, acc.z * il, acc.w * il));
-}
-
 template <bool READ>
 cudaError_t rows_op(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                     const KvTensor& v, int type, cudaStream_t stream) {
@@ -153,12 +86,12 @@ cudaError_t launch_kv_read(const KvArgs& c, const KvRows& r, int layer, const Kv
                            const KvTensor& v, int type, cudaStream_t stream) {
   return rows_op<true>(c, r, layer, k, v, type, stream);
 }
+// Few rows per sequence: the kernel that gives each its own CTA or cluster and
+// streams the cache once per row; more: tiles of rows on the tensor cores.
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream) {
   if (r.rows == 0) return cudaSuccess;
-  if (r.max_rows <= 8) return launch_kv_step(c, r, a, stream);
-  return launch(k_kv_attend_simple, dim3((unsigned)a.q_heads, (unsigned)((r.rows + 3) / 4)),
-                dim3(128), 0, stream, c, r, a);
+  return r.max_rows <= 8 ? launch_kv_step(c, r, a, stream) : launch_kv_tiles(c, r, a, stream);
 }
 
 }  // namespace qtts

@@ -17,6 +17,7 @@ ordered: one stream, or events between streams.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
 from . import engine as _e
@@ -34,9 +35,10 @@ class _Cache(C.Structure):
                 ("bits", C.c_int32)]
 
 
-class _Rows(C.Structure):
-    _fields_ = [("seqs", C.c_void_p), ("row_start", C.c_void_p), ("groups", C.c_int32),
-                ("rows", C.c_int32), ("max_rows", C.c_int32), ("max_length", C.c_int32)]
+# qtts_kv_rows: seqs, row_start, groups, rows, max_rows, max_length. Packed
+# bytes, one object per call (calls may come from several threads); making a
+# ctypes structure costs three times as much.
+_ROWS = struct.Struct("@PPiiii")
 
 
 def _invalid(message: str):
@@ -135,22 +137,22 @@ class KvCache:
                 t.record_stream(cur)
         return s
 
-    def _dtype(self, t, name: str, heads: Optional[int] = None) -> int:
+    def _tensor(self, t, name: str, heads: Optional[int] = None):
+        """Checks a row tensor; its dtype code, rows, heads and strides."""
         torch = self._torch
         d = t.dtype
         code = F32 if d is torch.float32 else BF16 if d is torch.bfloat16 else -1
         if code < 0:
             _invalid(f"{name} must be float32 or bfloat16, got {d}")
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+        shape, st = t.shape, t.stride()
+        if len(st) != 3 or shape[2] != HEAD_DIM or st[2] != 1:
             _invalid(f"{name} must be [rows, heads, {HEAD_DIM}] with a contiguous last dimension, "
-                     f"got shape {tuple(t.shape)} and strides {t.stride()}")
-        if t.stride(0) < 0 or t.stride(1) < 0:
-            _invalid(f"{name} has a negative stride")
-        if heads is not None and t.shape[1] != heads:
-            _invalid(f"{name} has {t.shape[1]} heads, the cache {heads}")
+                     f"got shape {tuple(shape)} and strides {st}")
+        if heads is not None and shape[1] != heads:
+            _invalid(f"{name} has {shape[1]} heads, the cache {heads}")
         if t.device != self.device:
             _invalid(f"{name} is on {t.device}, the cache on {self.device}")
-        return code
+        return code, shape[0], shape[1], st[0], st[1]
 
     def _index_array(self, t, name: str) -> int:
         if t.dtype is not self._torch.int32 or t.dim() != 1 or not t.is_contiguous():
@@ -159,10 +161,8 @@ class KvCache:
             _invalid(f"{name} is on {t.device}, the cache on {self.device}")
         return t.data_ptr()
 
-    def _rows(self, rows: int, seqs, row_start, max_rows: int, max_length: int):
-        if not 0 <= rows <= _INT_MAX:
-            _invalid(f"rows must be between 0 and {_INT_MAX}, got {rows}")
-        groups, starts, named = rows, None, None
+    def _rows(self, rows: int, seqs, row_start, max_rows: int, max_length: int) -> bytes:
+        groups, starts, named = rows, 0, 0
         if row_start is not None:
             starts = self._index_array(row_start, "row_start")
             groups = row_start.shape[0] - 1
@@ -172,21 +172,24 @@ class KvCache:
             named = self._index_array(seqs, "seqs")
             if seqs.shape[0] != groups:
                 _invalid(f"seqs names {seqs.shape[0]} sequences for {groups} groups of rows")
-        return C.byref(_Rows(named, starts, groups, rows, _int(max_rows, "max_rows"),
-                             _int(max_length, "max_length")))
+        try:
+            return _ROWS.pack(named, starts, groups, rows, max_rows, max_length)
+        except struct.error:
+            _invalid(f"rows ({rows}), max_rows ({max_rows}) and max_length ({max_length}) must be "
+                     "32-bit integers")
 
     def append(self, layer: int, k, v, *, seqs=None, row_start=None, max_rows: int = 0) -> None:
         """Stores rows ``k``, ``v`` [rows, kv_heads, 128]: group i (one row,
         or rows ``row_start[i]`` .. ``row_start[i + 1] - 1``) are the last rows
         of sequence ``seqs[i]`` (default i), whose length counts them already
         (``resize``)."""
-        dt = self._dtype(k, "k", self.kv_heads)
-        if self._dtype(v, "v", self.kv_heads) != dt or v.shape != k.shape:
+        dt, rows, _, k_row, k_head = self._tensor(k, "k", self.kv_heads)
+        dv, rows_v, _, v_row, v_head = self._tensor(v, "v", self.kv_heads)
+        if dv != dt or rows_v != rows:
             _invalid("k and v must have the same shape and dtype")
-        rows = self._rows(k.shape[0], seqs, row_start, max_rows, 0)
         _e._check(self._lib.qtts_kv_append(
-            self._ref, _int(layer, "layer"), rows, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), dt, self._stream()))
+            self._ref, _int(layer, "layer"), self._rows(rows, seqs, row_start, max_rows, 0),
+            k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, dt, self._stream()))
 
     def read(self, layer: int, rows: int, *, dtype=None, seqs=None, row_start=None,
              max_rows: int = 0):
@@ -197,6 +200,8 @@ class KvCache:
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in (torch.float32, torch.bfloat16):
             _invalid(f"dtype must be float32 or bfloat16, got {dtype}")
+        if rows < 0:
+            _invalid(f"rows must not be negative, got {rows}")
         groups = self._rows(rows, seqs, row_start, max_rows, 0)
         kv = torch.empty((2, rows, self.kv_heads, HEAD_DIM), dtype=dtype, device=self.device)
         half = rows * self.kv_heads * HEAD_DIM * kv.element_size()
@@ -216,17 +221,19 @@ class KvCache:
         ``max_rows`` and ``max_length`` only help the launch's shape. Rows that
         see nothing give zeros; rows outside every group are left as they are
         (undefined when ``out`` is not given)."""
-        dt = self._dtype(q, "q")
+        dt, rows, heads, q_row, q_head = self._tensor(q, "q")
         if out is None:
-            out = self._torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif self._dtype(out, "out") != dt or out.shape != q.shape:
-            _invalid("out must have q's shape and dtype")
-        rows = self._rows(q.shape[0], seqs, row_start, max_rows, max_length)
+            out = self._torch.empty_like(q)
+            o_row, o_head, _ = out.stride()
+        else:
+            do, rows_o, heads_o, o_row, o_head = self._tensor(out, "out")
+            if (do, rows_o, heads_o) != (dt, rows, heads):
+                _invalid("out must have q's shape and dtype")
         _e._check(self._lib.qtts_kv_attend(
-            self._ref, _int(layer, "layer"), rows, q.data_ptr(), q.stride(0), q.stride(1),
-            out.data_ptr(), out.stride(0), out.stride(1), dt, q.shape[1],
-            HEAD_DIM ** -0.5 if scale is None else scale, _int(window, "window"),
-            _int(sinks, "sinks"), self._stream()))
+            self._ref, _int(layer, "layer"),
+            self._rows(rows, seqs, row_start, max_rows, max_length), q.data_ptr(), q_row, q_head,
+            out.data_ptr(), o_row, o_head, dt, heads, HEAD_DIM ** -0.5 if scale is None else scale,
+            _int(window, "window"), _int(sinks, "sinks"), self._stream()))
         return out
 
     # ---- pages

@@ -34,13 +34,14 @@ def cache(kv, **over):
 def rows(kv, **over):
     f = dict(seqs=None, row_start=None, groups=0, rows=0, max_rows=0, max_length=0)
     f.update(over)
-    return kv._Rows(*[f[n] for n, _ in kv._Rows._fields_])
+    order = ("seqs", "row_start", "groups", "rows", "max_rows", "max_length")
+    return kv._ROWS.pack(*[f[n] or 0 for n in order])
 
 
 def attend(pkg, kv, c=None, r=None, layer=0, q=P, out=P, dtype=0, heads=2, scale=0.1, window=0,
            sinks=0, stride=128):
     return pkg.lib().qtts_kv_attend(
-        C.byref(c) if c is not None else None, layer, C.byref(r) if r is not None else None, q,
+        C.byref(c) if c is not None else None, layer, r, q,
         2 * stride, stride, out, 2 * stride, stride, dtype, heads, scale, window, sinks, None)
 
 
@@ -96,13 +97,13 @@ def test_append_and_read_refusals(pkg, kv):
     L = pkg.lib()
     for f in (L.qtts_kv_append, L.qtts_kv_read):
         r, c = rows(kv, groups=1, rows=1), cache(kv)
-        a = [C.byref(c), 0, C.byref(r), P, 256, 128, P, 256, 128, 0, None]
+        a = [C.byref(c), 0, r, P, 256, 128, P, 256, 128, 0, None]
         for i, bad, words in ((1, 2, "layer"), (3, None, "k"), (6, None, "v"), (9, 7, "dtype"),
                               (6, P + 1, "aligned")):
             refused(pkg, f(*[bad if j == i else x for j, x in enumerate(a)]), words)
         # no rows: nothing to do, nothing refused
         r = rows(kv)
-        assert f(C.byref(c), 0, C.byref(r), None, 0, 0, None, 0, 0, 0, None) == 0
+        assert f(C.byref(c), 0, r, None, 0, 0, None, 0, 0, 0, None) == 0
 
 
 def ints(*v):
