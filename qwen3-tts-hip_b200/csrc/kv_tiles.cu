@@ -7,24 +7,25 @@
 // of 64 (sinks first, then the window): S = Q K^T (128 x 64, two buffers in
 // TMEM), a thread per row turns its 64 scores into weights P with a running
 // maximum and sum, and O += P V (128 x 128, TMEM). Everything between is in
-// shared memory as K-major operands in the 128-byte swizzle.
+// shared memory in the 128-byte swizzle; V is the transposed operand, so K and
+// V keep the pages' own order of rows.
 //
-// Warps: 0-3 softmax and output (thread = matrix row = TMEM lane), 4-7 bring
-// blocks from the pages (16-bit K straight to shared memory by cp.async; the
-// rest through registers, two blocks in flight: V is transposed by byte
-// permutes, codes become values), 8 issues the matrix instructions. Nine warps
-// leave 168 registers a thread; thirteen (two groups of loaders) leave 128,
-// which spilled.
+// Four warpgroups: two of softmax (thread = matrix row = TMEM lane), which
+// take alternate blocks with statistics and an O of their own that are merged
+// at the end, so that one's exponentials hide the other's waits; one that
+// brings blocks from the pages (16 bits: cp.async, blocks ahead; 4 bits:
+// through registers, two blocks in flight, codes become values); one whose
+// first warp issues the matrix instructions. Registers are moved from the last
+// two to the first two.
 //
-// Number forms. 16-bit pages: bf16 operands as they are; rows of bf16 take Q
-// as it is and P as two bf16 parts (16 bits: one part would add an error of
-// the size of the output's own rounding); fp32 rows take Q and P as three
-// bf16 parts (24 bits). 4-bit pages: fp16 operands. A code times its bf16
-// scale has 11 significant bits, so it is exact in fp16 for scales of 2^-14 to
-// 2^12; queries are scaled per row by a power of two into fp16's range; P is
-// rounded to fp16 (2^-12), fp32 rows take two parts of each (22 bits). Scales
-// outside that range, and NaN or infinity in places that only some of the
-// rows see, send the CTA's rows to the row-by-row form (kv_attend_row).
+// Number forms. 16-bit pages, bf16 rows: Q K^T in bf16 as it is; P in fp16
+// (2^-12) with V in fp16, which holds a bf16 value exactly from 2^-14 to 2^16.
+// 16-bit pages, fp32 rows: Q and P as three bf16 parts (24 bits). 4-bit pages:
+// a code times its bf16 scale has 11 significant bits, so it is exact in fp16
+// for scales of 2^-14 to 2^12; queries are scaled per row by a power of two
+// into fp16's range; fp32 rows take Q and P as two fp16 parts (22 bits).
+// Values outside fp16's range, and NaN or infinity in places that only some
+// of the rows see, send the CTA's rows to the row-by-row form (kv_attend_row).
 //
 // The running maximum is raised only when a row's score exceeds it by more
 // than 2^8 (the weights then stay below 256, no trouble for fp32 sums), so
@@ -44,26 +45,35 @@ namespace {
 
 constexpr int kRowsM = 128;   // matrix rows of a CTA
 constexpr int kKeys = 64;     // positions per block
-constexpr int kLoadGroup = 128;  // loader threads
-constexpr int kMmaWarp = 8;
-constexpr int kTileThreads = 128 + kLoadGroup + 32;
-constexpr unsigned long long kTileWaitNs = 2000000000ull;
+constexpr int kGroup = 128;   // threads of a warpgroup
+constexpr int kTileThreads = 4 * kGroup;
+constexpr int kMmaWarp = 12;
+// Registers per thread of the warpgroups (128 at launch): they add up to 512.
+constexpr int kRegsSoftmax = 176, kRegsLoad = 112, kRegsMma = 48;
+static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * 128, "registers the block was given");
+constexpr long long kTileWaitCycles = 4000000000ll;  // two seconds at 2 GHz
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int BITS, bool F32>
 struct Form {
-  static constexpr int qp = !F32 ? 1 : BITS == 16 ? 3 : 2;                   // parts of Q
-  static constexpr int pp = BITS == 16 ? (F32 ? 3 : 2) : (F32 ? 2 : 1);     // parts of P
+  static constexpr bool qk16 = BITS == 4;           // Q and K in fp16 (else bf16)
+  static constexpr bool pv16 = !(BITS == 16 && F32);  // P and V in fp16
+  static constexpr int qp = !F32 ? 1 : BITS == 16 ? 3 : 2;  // parts of Q
+  static constexpr int pp = qp;                             // parts of P
+  // softmax warpgroups at work: shared memory has no room for two P of three parts
+  static constexpr int groups = BITS == 16 && F32 ? 1 : 2;
   static constexpr int q_bytes = qp * kRowsM * kKvDim * 2;
   static constexpr int p_bytes = pp * kRowsM * kKeys * 2;
   static constexpr int kv_bytes = kKeys * kKvDim * 2;          // K or V of one block
-  static constexpr int stages = F32 && BITS == 16 ? 2 : 3;
-  static constexpr int smem = q_bytes + p_bytes + stages * 2 * kv_bytes + 1024;
-  static_assert(smem <= 227 * 1024, "shared memory of one SM");
+  static constexpr int stages = F32 ? 2 : 4;
+  static constexpr int smem = q_bytes + groups * p_bytes + stages * 2 * kv_bytes + 1024;
+  static_assert(smem + 2304 <= 227 * 1024, "shared memory of one SM");
 };
 
+constexpr int kMaxStages = 4;
 struct Bars {
-  uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2], sempty[2], pfull, pempty, done;
+  uint64_t kfull[kMaxStages], kempty[kMaxStages], vfull[kMaxStages], vempty[kMaxStages];
+  uint64_t sfull[2], sempty[2], pfull[2], pempty[2], done;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -71,9 +81,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <int BITS>
+template <bool HALF>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  if constexpr (BITS == 16) {
+  if constexpr (!HALF) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   } else {
@@ -81,16 +91,11 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-template <int BITS>
-__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
-  if constexpr (BITS == 16) return make_float2(bf16lo(w), bf16hi(w));
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
 // Byte of 16-byte chunk `ch` (0..7) of row `r` in a [rows][64] swizzled tile.
 __device__ __forceinline__ int swz(int r, int ch) { return r * 128 + ((ch ^ (r & 7)) << 4); }
 
 // Eight values as `PARTS` operands of 16 bits, each what the ones before left.
-template <int BITS, int PARTS>
+template <bool HALF, int PARTS>
 __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[PARTS]) {
   float r[8];
 #pragma unroll
@@ -100,9 +105,17 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[PARTS])
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = pack_pair<BITS>(r[2 * i], r[2 * i + 1]);
+      if (!HALF && p + 1 < PARTS) {
+        // cut, not rounded: one permute, and the next part takes the rest
+        const uint32_t a = __float_as_uint(r[2 * i]), b = __float_as_uint(r[2 * i + 1]);
+        w[i] = __byte_perm(a, b, 0x7632);
+        r[2 * i] -= __uint_as_float(a & 0xffff0000u);
+        r[2 * i + 1] -= __uint_as_float(b & 0xffff0000u);
+        continue;
+      }
+      w[i] = pack_pair<HALF>(r[2 * i], r[2 * i + 1]);
       if (p + 1 < PARTS) {
-        const float2 f = unpack_pair<BITS>(w[i]);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         r[2 * i] -= f.x;
         r[2 * i + 1] -= f.y;
       }
@@ -111,13 +124,14 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[PARTS])
   }
 }
 
-// What loaders meet in a tile's blocks. 4-bit scales: below 2^-14 (tiny) a
-// product is rounded to multiples of 2^-24, which matters only where no scale
-// of 2^-8 or more (big) sets the size of the values.
-enum : int { kOdd = 1, kTinyK = 2, kBigK = 4, kTinyV = 8, kBigV = 16 };
+// What loaders meet in a tile's blocks: odd values (NaN, infinity, past fp16);
+// and whether what fp16 rounds (below 2^-14, to multiples of 2^-24) is small
+// beside the rest: some K, some V of at least 2^-11 (a scale for 4 bits), or
+// nothing but zeros.
+enum : int { kOdd = 1, kAnyK = 2, kBigK = 4, kAnyV = 8, kBigV = 16 };
 __device__ __forceinline__ bool row_by_row(int seen) {
-  return (seen & kOdd) || ((seen & kTinyK) && !(seen & kBigK)) ||
-         ((seen & kTinyV) && !(seen & kBigV));
+  return (seen & kOdd) || ((seen & kAnyK) && !(seen & kBigK)) ||
+         ((seen & kAnyV) && !(seen & kBigV));
 }
 
 // The group of blockIdx.x: its rows and sequence. Same checks as kv_place.
@@ -148,112 +162,388 @@ __device__ __forceinline__ bool group_rows(const KvArgs& c, const KvRows& r, int
   return true;
 }
 
-// One block of 64 positions in a loader thread's registers.
-template <int BITS>
-struct Block;
-template <>
-struct Block<16> {
-  uint4 v[8];       // keys 8 kb + i, dims 8 db ..
+// 4 bits: one block of 64 positions in a loader thread's registers. K and V:
+// row krow + 8 i, the word of dims 8 kch .. and (bf16, low half) its scale.
+struct Codes {
+  uint32_t k[8], ks[8], v[8], vs[8];
 };
-template <>
-struct Block<4> {
-  uint32_t k[8];    // K: dims 8 per word, row lt / 16 + 8 i
-  uint32_t ks[8];   // the scale of that group, bf16 in the low half
-  uint32_t v[8];    // V: keys 8 kb + i, dims 8 db ..
-  uint32_t vs[8];
+
+template <int REGS, bool MORE>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (MORE)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int ID, int THREADS>
+__device__ __forceinline__ void bar() {
+  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory");
+}
+
+// The row tiles of one CTA, the same for every role.
+struct Walk {
+  int begin, end, len, rows_per, window, sinks;
+  int row0, n, pos0, last, ns, ws, blocks;
+
+  __device__ __forceinline__ void tile(int t) {
+    row0 = begin + t * rows_per;
+    n = min(rows_per, end - row0);
+    pos0 = len - (end - row0);              // position of the tile's first row
+    last = len < 0 ? -1 : pos0 + n - 1;     // < 0: no row holds a position
+    // blocks that some row sees: [0, ns) and [ws, last / 64]
+    const KvSpan lo = kv_span(max(pos0, 0), window, sinks), hi = kv_span(max(last, 0), window, sinks);
+    ns = (hi.sink_end + kKeys - 1) / kKeys;
+    ws = max(lo.first / kKeys, ns);
+    blocks = last < 0 ? 0 : ns + max(0, last / kKeys - ws + 1);
+  }
+  __device__ __forceinline__ int block_pos(int j) const { return (j < ns ? j : j - ns + ws) * kKeys; }
+  // every row sees every position of the block at p0
+  __device__ __forceinline__ bool whole(int p0) const {
+    return pos0 >= 0 && p0 + kKeys - 1 <= pos0 &&
+           (window == 0 || p0 > last - window || p0 + kKeys <= sinks);
+  }
+  // Pages of the quarters of eight blocks, one per lane (a page is at least a
+  // quarter), read together when the first of them is wanted.
+  __device__ __forceinline__ void refill(const KvArgs& c, int seq, int j, int& held) const {
+    const int lane = threadIdx.x & 31, jj = (j & ~7) + (lane >> 2);
+    const int p = block_pos(jj) + 16 * (lane & 3);
+    held = jj < blocks && p <= last ? kv_page(c, seq, p >> c.g.shift) : -1;
+  }
 };
 
 template <int BITS, bool F32>
 __global__ void __launch_bounds__(kTileThreads, 1)
     k_kv_tiles(KvArgs c, KvRows r, KvAttend a, int chunks, int gheads, int rows_per, int tiles) {
   using Fm = Form<BITS, F32>;
-  constexpr int QP = Fm::qp, PP = Fm::pp, ST = Fm::stages;
+  constexpr int QP = Fm::qp, PP = Fm::pp, ST = Fm::stages, NG = Fm::groups;
   extern __shared__ uint8_t tile_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(tile_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
-  uint8_t* sp = sq + Fm::q_bytes;
-  uint8_t* skv = sp + Fm::p_bytes;  // stage s: K at 2 s, V at 2 s + 1 (kv_bytes each)
+  uint8_t* sp = sq + Fm::q_bytes;                 // NG buffers
+  uint8_t* skv = sp + NG * Fm::p_bytes;           // stage s: K at 2 s, V at 2 s + 1 (kv_bytes each)
   __shared__ Bars b;
   __shared__ uint32_t s_tmem;
   __shared__ int s_seen;  // what the loaders met (kOdd ..)
   __shared__ int s_dead;  // a wait ran out
+  __shared__ float s_top[2][kRowsM], s_sum[2][kRowsM];
 
   pdl_wait();
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = blockIdx.x % r.groups;
   const int head = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
   const int per_head = a.q_heads / c.g.kv_heads;
   const int heads = min(gheads, per_head - chunk * gheads);
   const int qh0 = head * per_head + chunk * gheads;
-  int seq, begin, end, len;
-  if (!group_rows(c, r, group, &seq, &begin, &end, &len)) return;
+  Walk w;
+  int seq;
+  if (!group_rows(c, r, group, &seq, &w.begin, &w.end, &w.len)) return;
   if (a.halt && __ldcg(a.halt + (long long)group * a.halt_stride)) return;
+  w.rows_per = rows_per;
+  w.window = a.window;
+  w.sinks = a.sinks;
+  // tiles with more positions first; more row tiles than the launch was told
+  // of are taken in turn
+  const int tile0 = tiles - 1 - (int)(blockIdx.x / r.groups);
+  auto more = [&](int t) { return (long long)t * rows_per < w.end - w.begin; };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&b.kfull[i], kLoadGroup / 32);
-      mbar_init(&b.vfull[i], kLoadGroup / 32);
+      mbar_init(&b.kfull[i], kGroup / 32);
+      mbar_init(&b.vfull[i], kGroup / 32);
       mbar_init(&b.kempty[i], 1);
       mbar_init(&b.vempty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.sfull[i], 1);
       mbar_init(&b.sempty[i], 4);
+      mbar_init(&b.pfull[i], 4);
+      mbar_init(&b.pempty[i], 1);
     }
-    mbar_init(&b.pfull, 4);
-    mbar_init(&b.pempty, 1);
     mbar_init(&b.done, 1);
     fence_mbar_init();
     s_dead = 0;
+    s_seen = 0;
   }
-  if (warp == kMmaWarp) tmem_alloc(&s_tmem, 256);
+  if (warp == kMmaWarp) tmem_alloc(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm_s = s_tmem, tm_o = s_tmem + 128;
+  // Dependents may start once every CTA holds its TMEM: one that took columns
+  // first and then waited for this grid would never let it finish.
+  pdl_trigger();
+  const uint32_t tm_s = s_tmem, tm_o = s_tmem + 2 * kKeys;  // O of group w at + 128 w
 
-  // bounded waits: of one thread, and of a warp (all lanes give up together)
+  // Bounded waits of a warp: all lanes give up together.
   auto wait = [&](uint64_t* bar, unsigned parity) {
-    if (mbar_wait_ns(bar, parity & 1, kTileWaitNs)) return true;
-    atomicExch(&s_dead, 1);
-    return false;
+    const bool ok = mbar_wait_cycles(bar, parity & 1, kTileWaitCycles);
+    if (!ok) atomicExch(&s_dead, 1);
+    return __all_sync(0xffffffffu, ok) != 0;
   };
-  auto wait_warp = [&](uint64_t* bar, unsigned parity) {
-    return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
-  };
+  // Per row tile, every role: bar 0 (Q is in place), its blocks, bar 0 (all are
+  // done with the tile). `base`: blocks of the tiles before (stages and phases
+  // run on). After a wait ran out the tiles that are left are skipped.
+  int base = 0;
 
-  int base = 0;        // blocks of the tiles before this one (stage and phase run on)
-  unsigned dones = 0;  // tiles finished
-  // more row tiles than the launch was told of are taken in turn
-  for (int tile = tiles - 1 - (int)(blockIdx.x / r.groups); tile * rows_per < end - begin;
-       tile += tiles) {
-    const int row0 = begin + tile * rows_per;
-    const int n = min(rows_per, end - row0);
-    const int pos0 = len - (end - row0);            // position of the tile's first row
-    const int last = len < 0 ? -1 : pos0 + n - 1;   // < 0: no row holds a position
-    const int low = max(pos0, 0);
-    // blocks that some row sees: [0, ns) and [ws, last / 64]
-    const KvSpan s_lo = kv_span(low, a.window, a.sinks), s_hi = kv_span(max(last, 0), a.window, a.sinks);
-    const int ns = (s_hi.sink_end + kKeys - 1) / kKeys;
-    const int ws = max(s_lo.first / kKeys, ns);
-    const int blocks = last < 0 ? 0 : ns + max(0, last / kKeys - ws + 1);
-    auto block_pos = [&](int j) { return (j < ns ? j : j - ns + ws) * kKeys; };
-    // every row sees every position of the block
-    auto whole = [&](int p0) {
-      return pos0 >= 0 && p0 + kKeys - 1 <= pos0 &&
-             (a.window == 0 || p0 > last - a.window || p0 + kKeys <= a.sinks);
-    };
-    if (threadIdx.x == 0) s_seen = 0;
-    float q_scale = 1.f;  // softmax threads: what undoes the row's power of two
-    if (warp < 4) {
-      // ---- Q: this thread's matrix row
-      const int m = threadIdx.x, rr = m / heads, hh = m - rr * heads;
-      const bool in = rr < n;
-      const long long off = (long long)(row0 + rr) * a.q.row + (long long)(qh0 + hh) * a.q.head;
+  if (warp >= kMmaWarp) {
+    // ---- matrix instructions: the warp walks together (its operands stay in
+    // uniform registers), one lane issues
+    set_registers<kRegsMma, false>();
+    constexpr uint32_t is = Fm::qk16 ? umma_idesc_f16(kRowsM, kKeys) : umma_idesc_bf16(kRowsM, kKeys);
+    constexpr uint32_t io = (Fm::pv16 ? umma_idesc_f16(kRowsM, kKvDim) : umma_idesc_bf16(kRowsM, kKvDim)) |
+                            kUmmaTransposeB;
+    const uint64_t dq = umma_desc_sw128(sq), dp = umma_desc_sw128(sp), dkv = umma_desc_sw128(skv),
+                   dvt = umma_desc_sw128_mn(skv, kKeys * 128);
+    for (int t = tile0; more(t); t += tiles) {
+      w.tile(t);
+      bar<0, kTileThreads>();
+      if (warp == kMmaWarp) {
+        auto scores = [&](int j) {
+          const int g = base + j, s = g % ST;
+          if (!wait(&b.kfull[s], g / ST) || !wait(&b.sempty[g & 1], (g >> 1) + 1)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int p = 0; p < QP; ++p)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)  // halves of 64 dims, four steps of 32 bytes in each
+                umma_bf16(tm_s + (g & 1) * kKeys,
+                          dq + (((2 * p + (k >> 2)) * (kRowsM * 128)) >> 4) + 2 * (k & 3),
+                          dkv + ((2 * s * Fm::kv_bytes + (k >> 2) * (kKeys * 128)) >> 4) + 2 * (k & 3),
+                          is, (p | k) != 0);
+            umma_commit(&b.kempty[s]);
+            umma_commit(&b.sfull[g & 1]);
+          }
+          __syncwarp();
+          return true;
+        };
+        bool fine = (w.blocks < 1 || scores(0)) && (w.blocks < 2 || scores(1));
+        for (int j = 0; j < w.blocks && fine; ++j) {
+          const int g = base + j, s = g % ST, wg = g % NG;
+          if (!wait(&b.vfull[s], g / ST) || !wait(&b.pfull[wg], g / NG)) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int p = 0; p < PP; ++p)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_bf16(tm_o + wg * kKvDim, dp + ((wg * Fm::p_bytes + p * (kRowsM * 128)) >> 4) + 2 * k,
+                          dvt + (((2 * s + 1) * Fm::kv_bytes + k * 16 * 128) >> 4), io,
+                          j >= NG || (p | k) != 0);
+            umma_commit(&b.vempty[s]);
+            umma_commit(&b.pempty[wg]);
+          }
+          __syncwarp();
+          fine = j + 2 >= w.blocks || scores(j + 2);
+        }
+        // the output is read, and the next tile begun, after every product
+        if (elect_one()) umma_commit(&b.done);
+        __syncwarp();
+      }
+      base += w.blocks;
+      bar<0, kTileThreads>();
+      if (s_dead) break;
+    }
+    tc_fence_before();
+    bar<0, kTileThreads>();
+    tc_fence_after();
+    if (warp == kMmaWarp) {
+      if (lane == 0 && s_dead) kv_status(c, kKvTimeout);
+      tmem_free(s_tmem, 512);
+    }
+    return;
+  }
+
+  if (warp >= 8) {
+    // ---- loaders
+    set_registers<kRegsLoad, false>();
+    const int lt = threadIdx.x - 2 * kGroup;
+    const int krow = lt >> 4, kch = lt & 15;      // rows krow + 8 i, dims 8 kch ..
+    const long long page_bytes = kv_page_bytes(c.g);
+    const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
+    const long long v_off = kv_tile_bytes(c.g) * c.g.kv_heads;  // from K's tile to V's
+    const int mask = (1 << c.g.shift) - 1;
+    const int at0 = (kch >> 3) * (kKeys * 128) + swz(krow, kch & 7);  // row krow + 8 i: + 1024 i
+    for (int t = tile0; more(t); t += tiles) {
+      w.tile(t);
+      bar<0, kTileThreads>();
+      int seen = 0;
+      if constexpr (BITS == 16) {
+        // Copies: group a holds K of block a + 1 and V of block a (K first: its
+        // product comes earlier), group -1 K of block 0. They are started ST - 2
+        // groups ahead; positions that are not there become 0.
+        int held[2] = {-1, -1};
+        auto start = [&](int j, int which) {  // block j, 0: K, 1: V
+          if (j >= w.blocks) return true;
+          const int g = base + j, s = g % ST, p0 = w.block_pos(j);
+          if ((j & 7) == 0) w.refill(c, seq, j, held[which]);
+          if (!wait(which ? &b.vempty[s] : &b.kempty[s], g / ST + 1)) return false;
+          const uint32_t dst = smem_u32(skv + (2 * s + which) * Fm::kv_bytes) + at0;
+          const unsigned char* from = kbase + (which ? v_off : 0) + krow * 256 + kch * 16;
+#pragma unroll
+          for (int qu = 0; qu < 4; ++qu) {
+            const int page = __shfl_sync(0xffffffffu, held[which], 4 * (j & 7) + qu);
+            const int p = p0 + 16 * qu;
+            const unsigned char* src = from + max(page, 0) * page_bytes + (p & mask) * 256;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool ok = page >= 0 && p + krow + 8 * h <= w.last;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 2048 * qu + 1024 * h),
+                           "l"(src + 2048 * h), "r"(ok ? 16 : 0)
+                           : "memory");
+            }
+          }
+          return true;
+        };
+        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+        auto give = [&](uint64_t* full) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        };
+        unsigned top = 0u;  // largest magnitudes of V, per half word
+        bool fine = start(0, 0);
+        commit();
+        for (int i = 0; i < ST - 2 && fine; ++i) {
+          fine = start(i + 1, 0) && start(i, 1);
+          commit();
+        }
+        if (fine && w.blocks > 0) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+          give(&b.kfull[base % ST]);
+        }
+        for (int j = 0; j < w.blocks && fine; ++j) {
+          if constexpr (ST == 2) {  // nothing ahead: started now
+            fine = start(j + 1, 0) && start(j, 1);
+            commit();
+            if (!fine) break;
+          }
+          asm volatile("cp.async.wait_group %0;" ::"n"(ST >= 3 ? ST - 3 : 0) : "memory");
+          if (j + 1 < w.blocks) give(&b.kfull[(base + j + 1) % ST]);
+          const int s = (base + j) % ST;
+          uint8_t* sv = skv + (2 * s + 1) * Fm::kv_bytes + at0;
+          // pv16: bf16 becomes fp16, and the largest magnitude says whether it fits;
+          // else only NaN or infinity where some rows look and others do not matters
+          if (Fm::pv16 || !w.whole(w.block_pos(j))) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint4 v = *reinterpret_cast<const uint4*>(sv + 1024 * i);
+              top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                           __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+              if constexpr (Fm::pv16) {
+                v.x = pack_pair<true>(bf16lo(v.x), bf16hi(v.x));
+                v.y = pack_pair<true>(bf16lo(v.y), bf16hi(v.y));
+                v.z = pack_pair<true>(bf16lo(v.z), bf16hi(v.z));
+                v.w = pack_pair<true>(bf16lo(v.w), bf16hi(v.w));
+                *reinterpret_cast<uint4*>(sv + 1024 * i) = v;
+              }
+            }
+          }
+          give(&b.vfull[s]);
+          if constexpr (ST > 2) {
+            fine = start(j + ST - 1, 0) && start(j + ST - 2, 1);
+            commit();
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        const unsigned m = max(top & 0xffffu, top >> 16);
+        // bf16 bits: 0x7f80 infinity; fp16 ends below 2^16 (0x4780); 2^-11 is 0x3a00
+        seen = m >= (Fm::pv16 ? 0x4780u : 0x7f80u) ? kOdd : 0;
+        if (Fm::pv16) seen |= (m ? kAnyV : 0) | (m >= 0x3a00u ? kBigV : 0);
+      } else {
+        int held = -1;
+        auto load = [&](Codes& x, int j) {
+          const int p0 = w.block_pos(j);
+          if ((j & 7) == 0) w.refill(c, seq, j, held);
+          const unsigned char* from = kbase + krow * 64 + kv_code_word_at(8 * kch);
+          const unsigned char* from_s = kbase + (kKvCodeBytes << c.g.shift) + krow * 8 + 2 * (kch >> 2);
+#pragma unroll
+          for (int qu = 0; qu < 4; ++qu) {
+            const int page = __shfl_sync(0xffffffffu, held, 4 * (j & 7) + qu);
+            const int p = p0 + 16 * qu;
+            const long long at = max(page, 0) * page_bytes;
+            const unsigned char* src = from + at + (p & mask) * 64;
+            const unsigned char* src_s = from_s + at + (p & mask) * 8;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool ok = page >= 0 && p + krow + 8 * h <= w.last;
+              const int i = 2 * qu + h;
+              x.k[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(src + 512 * h)) : 0u;
+              x.v[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(src + v_off + 512 * h)) : 0u;
+              x.ks[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(src_s + 64 * h)) : 0u;
+              x.vs[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(src_s + v_off + 64 * h)) : 0u;
+            }
+          }
+        };
+        // Eight codes (one word) times their scale, in fp16, dims in order.
+        auto put = [&](uint8_t* dst, uint32_t x, uint32_t s16, int any, int big) {
+          const float s = __uint_as_float(s16 << 16);
+          seen |= (s <= 4096.f ? 0 : kOdd) | (s != 0.f ? any : 0) | (s >= 0.00048828125f ? big : 0);
+          const __half2 sc = __half2half2(__float2half_rn(s));
+          uint32_t o[4];  // pair i: nibbles i and i + 4
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = ((x >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
+            const __half2 n =
+                __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
+            const __half2 v = __hmul2(n, sc);
+            o[i] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          *reinterpret_cast<uint4*>(dst) =
+              make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
+                         __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
+        };
+        auto store = [&](const Codes& x, int j) {
+          const int g = base + j, s = g % ST;
+          uint8_t* sk = skv + 2 * s * Fm::kv_bytes + at0;
+          if (!wait(&b.kempty[s], g / ST + 1)) return false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) put(sk + 1024 * i, x.k[i], x.ks[i], kAnyK, kBigK);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.kfull[s]);
+          if (!wait(&b.vempty[s], g / ST + 1)) return false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            put(sk + Fm::kv_bytes + 1024 * i, x.v[i], x.vs[i], kAnyV, kBigV);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.vfull[s]);
+          return true;
+        };
+        Codes x, y;
+        if (w.blocks > 0) load(x, 0);
+        for (int j = 0; j < w.blocks; j += 2) {
+          if (j + 1 < w.blocks) load(y, j + 1);
+          if (!store(x, j) || j + 1 >= w.blocks) break;
+          if (j + 2 < w.blocks) load(x, j + 2);
+          if (!store(y, j + 1)) break;
+        }
+      }
+      if (seen) atomicOr(&s_seen, seen);
+      base += w.blocks;
+      bar<0, kTileThreads>();
+      if (s_dead) break;
+    }
+    bar<0, kTileThreads>();
+    return;
+  }
+
+  // ---- softmax: thread = matrix row
+  set_registers<kRegsSoftmax, true>();
+  const int wg = warp >> 2, m = threadIdx.x & (kGroup - 1);
+  const int rr = m / heads, hh = m - rr * heads;
+  const uint32_t quad = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
+  unsigned dones = 0;
+  for (int t = tile0; more(t); t += tiles) {
+    w.tile(t);
+    float q_scale = 1.f;  // what undoes the row's power of two
+    {
+      // Q: with two groups each stores half of the dims of its row
+      const bool in = rr < w.n;
+      const long long off = (long long)(w.row0 + rr) * a.q.row + (long long)(qh0 + hh) * a.q.head;
       float up = 1.f;
-      if constexpr (BITS == 4) {
+      if constexpr (Fm::qk16) {
         float top = 0.f;
         if (in)
 #pragma unroll 8
@@ -268,384 +558,165 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           q_scale = __uint_as_float((unsigned)(127 - 8 + e) << 23);
         }
       }
+      // a negative scale goes into Q, so that masked scores are -inf either way
+      if (a.scale < 0.f) up = -up;
 #pragma unroll 4
-      for (int ch = 0; ch < 16; ++ch) {
-        float x[8];
+      for (int ch = 8 * wg; ch < 8 * wg + 8; ++ch) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (in) {
           const float4 y = kv_load4(a.q.p, off + 8 * ch, a.type);
           const float4 z = kv_load4(a.q.p, off + 8 * ch + 4, a.type);
-          x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-          x[4] = z.x; x[5] = z.y; x[6] = z.z; x[7] = z.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+          x[0] = y.x * up; x[1] = y.y * up; x[2] = y.z * up; x[3] = y.w * up;
+          x[4] = z.x * up; x[5] = z.y * up; x[6] = z.z * up; x[7] = z.w * up;
         }
-        // a negative scale goes into Q, so that masked scores are -inf either way
-        const float u = a.scale < 0.f ? -up : up;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= u;
-        uint4 w[QP];
-        split8<BITS, QP>(x, w);
+        uint4 o[QP];
+        split8<Fm::qk16, QP>(x, o);
 #pragma unroll
         for (int p = 0; p < QP; ++p)
-          *reinterpret_cast<uint4*>(sq + (2 * p + (ch >> 3)) * (kRowsM * 128) + swz(m, ch & 7)) = w[p];
+          *reinterpret_cast<uint4*>(sq + (2 * p + (ch >> 3)) * (kRowsM * 128) + swz(m, ch & 7)) = o[p];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    __syncthreads();
-
-    if (warp == kMmaWarp) {
-      // ---- matrix instructions, one thread
-      if (lane == 0) {
-        constexpr uint32_t is = BITS == 16 ? umma_idesc_bf16(kRowsM, kKeys) : umma_idesc_f16(kRowsM, kKeys);
-        constexpr uint32_t io = BITS == 16 ? umma_idesc_bf16(kRowsM, kKvDim) : umma_idesc_f16(kRowsM, kKvDim);
-        bool ok = true;
-        auto scores = [&](int j) {
-          const int g = base + j, s = g % ST;
-          if (!wait(&b.kfull[s], g / ST) || !wait(&b.sempty[g & 1], (g >> 1) + 1)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int p = 0; p < QP; ++p)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint64_t dq = umma_desc_sw128(sq + (2 * p + h) * (kRowsM * 128));
-              const uint64_t dk = umma_desc_sw128(skv + 2 * s * Fm::kv_bytes + h * (kKeys * 128));
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_bf16(tm_s + (g & 1) * kKeys, dq + 2 * k, dk + 2 * k, is, (p | h | k) != 0);
-            }
-          umma_commit(&b.kempty[s]);
-          umma_commit(&b.sfull[g & 1]);
-          return true;
-        };
-        if (blocks) ok = scores(0);
-        for (int j = 0; j < blocks && ok; ++j) {
-          if (j + 1 < blocks && !scores(j + 1)) break;
-          const int g = base + j, s = g % ST;
-          if (!wait(&b.vfull[s], g / ST) || !wait(&b.pfull, g)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int p = 0; p < PP; ++p) {
-            const uint64_t dp = umma_desc_sw128(sp + p * (kRowsM * 128));
-            const uint64_t dv = umma_desc_sw128(skv + (2 * s + 1) * Fm::kv_bytes);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16(tm_o, dp + 2 * k, dv + 2 * k, io, j > 0 || (p | k) != 0);
-          }
-          umma_commit(&b.vempty[s]);
-          umma_commit(&b.pempty);
-        }
-        umma_commit(&b.done);
+    bar<0, kTileThreads>();
+    const int pos = rr < w.n ? w.pos0 + rr : -1;
+    // (a scale of 0 stays a positive factor: -inf * 0 is not a number)
+    const float f = fmaxf(fabsf(a.scale) * kLog2e * q_scale, 1.2e-38f);
+    float top = -INFINITY, sum = 0.f;  // top: in units of log2, of scaled scores
+    int held = -1, held_at = -1;
+    int first = NG == 1 ? 0 : (wg - base) & 1;  // this group's blocks: (base + j) % 2 == wg
+    if (wg >= NG) first = w.blocks;
+    for (int j = first; j < w.blocks; j += NG) {
+      const int g = base + j;
+      const int p0 = w.block_pos(j);
+      float x[kKeys];
+      if ((j >> 3) != held_at) {
+        held_at = j >> 3;
+        w.refill(c, seq, j, held);
       }
-    } else if (warp >= 4) {
-      // ---- loaders
-      const int lt = threadIdx.x - 128;
-      const int kb = lt & 7, db = lt >> 3;          // V: keys 8 kb .., dims 8 db ..
-      const int krow = lt >> 4, kch = lt & 15;      // K: rows krow + 8 i, dims 8 kch ..
-      const long long tile_bytes = kv_tile_bytes(c.g), page_bytes = kv_page_bytes(c.g);
-      const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
-      const unsigned char* vbase = kbase + tile_bytes * c.g.kv_heads;
-      const int mask = (1 << c.g.shift) - 1;
-      // pages of a block's four quarters (a page is at least one of them)
-      auto pages = [&](int p0, int (&pg)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = p0 + 16 * i;
-          pg[i] = p <= last ? kv_page(c, seq, p >> c.g.shift) : -1;
-        }
-      };
-      // 16 bits: K of block j to its stage; positions that are not there become 0
-      auto copy_k = [&](int j) {
-        const int g = base + j, s = g % ST, p0 = block_pos(j);
-        int pg[4];
-        pages(p0, pg);
-        if (!wait_warp(&b.kempty[s], g / ST + 1)) return false;
-        const uint32_t sk = smem_u32(skv + 2 * s * Fm::kv_bytes + (kch >> 3) * (kKeys * 128));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int kr = krow + 8 * i, page = pg[i >> 1];
-          const bool ok = page >= 0 && p0 + kr <= last;
-          const unsigned char* src =
-              kbase + (ok ? page : 0) * page_bytes + ((p0 + kr) & mask) * 256 + kch * 16;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sk + swz(kr, kch & 7)),
-                       "l"(src), "r"(ok ? 16 : 0)
-                       : "memory");
-        }
-        return true;
-      };
-      auto load = [&](Block<BITS>& x, int p0) {
-        int pg[4];
-        pages(p0, pg);
-        if constexpr (BITS == 4) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int kr = krow + 8 * i;             // in quarter i / 2
-            const int page = pg[i >> 1], prow = (p0 + kr) & mask;
-            const bool ok = page >= 0 && p0 + kr <= last;
-            const unsigned char* t = kbase + (ok ? page : 0) * page_bytes;
-            x.k[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(t + prow * 64 + kv_code_word_at(8 * kch)))
-                        : 0x88888888u;
-            x.ks[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(t + (kKvCodeBytes << c.g.shift)) +
-                                  prow * 4 + (kch >> 2))
-                         : 0u;
-          }
-        }
-        const int vq = kb >> 1;                      // the quarter of this thread's keys
-        const int vpage = vq == 0 ? pg[0] : vq == 1 ? pg[1] : vq == 2 ? pg[2] : pg[3];
-        const int prow0 = (p0 + 8 * kb) & mask;      // eight rows of one page
-        const unsigned char* t = vbase + max(vpage, 0) * page_bytes;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int prow = prow0 + i;
-          const bool ok = vpage >= 0 && p0 + 8 * kb + i <= last;
-          if constexpr (BITS == 16) {
-            x.v[i] = ok ? __ldcg(reinterpret_cast<const uint4*>(t + prow * 256) + db)
-                        : make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            x.v[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(t + prow * 64 + kv_code_word_at(8 * db)))
-                        : 0x88888888u;
-            x.vs[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(t + (kKvCodeBytes << c.g.shift)) +
-                                  prow * 4 + (db >> 2))
-                         : 0u;
-          }
-        }
-      };
-      // a 4-bit scale as fp16 (both halves)
-      int seen = 0;
-      auto half_scale = [&](uint32_t s16, int tiny, int big) {
-        const float s = __uint_as_float(s16 << 16);
-        seen |= (s <= 4096.f ? 0 : kOdd) | (s != 0.f && s < 6.103515625e-05f ? tiny : 0) |
-                (s >= 0.00390625f ? big : 0);
-        return __half2half2(__float2half_rn(s));
-      };
-      // eight codes (one word) times a scale: four words of two fp16 values,
-      // pair i = nibbles i and i + 4
-      auto values = [&](uint32_t w, __half2 s, uint32_t (&o)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
-          const __half2 nv = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
-          const __half2 v = __hmul2(nv, s);
-          o[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-      };
-      auto store = [&](Block<BITS>& x, int j) {
-        const int g = base + j, s = g % ST;
-        uint8_t* sk = skv + 2 * s * Fm::kv_bytes;
-        uint8_t* sv = sk + Fm::kv_bytes;
-        const int p0 = block_pos(j);
-        if constexpr (BITS == 16) {
-          // the copies of block j are the oldest of at most ST - 1 groups in flight
-          asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        } else {
-          if (!wait_warp(&b.kempty[s], g / ST + 1)) return false;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t o[4];
-            values(x.k[i], half_scale(x.ks[i], kTinyK, kBigK), o);
-            // dims in order: pairs (0, 1), (2, 3) from nibbles (i, i + 4)
-            *reinterpret_cast<uint4*>(sk + (kch >> 3) * (kKeys * 128) + swz(krow + 8 * i, kch & 7)) =
-                make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
-                           __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b.kfull[s]);
-        if (!wait_warp(&b.vempty[s], g / ST + 1)) return false;
-        if constexpr (BITS == 16) {
-          if (!whole(p0)) {
-            // NaN or infinity where only some rows look
-            uint32_t bad = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t w = k == 0 ? x.v[i].x : k == 1 ? x.v[i].y : k == 2 ? x.v[i].z : x.v[i].w;
-                bad |= ((w & 0x7f80u) == 0x7f80u) | ((w & 0x7f800000u) == 0x7f800000u);
-              }
-            if (bad) seen |= kOdd;
-          }
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const unsigned sel = d & 1 ? 0x7632u : 0x5410u;
-            auto at = [&](int i) {
-              return d / 2 == 0 ? x.v[i].x : d / 2 == 1 ? x.v[i].y : d / 2 == 2 ? x.v[i].z : x.v[i].w;
-            };
-            *reinterpret_cast<uint4*>(sv + swz(8 * db + d, kb)) =
-                make_uint4(__byte_perm(at(0), at(1), sel), __byte_perm(at(2), at(3), sel),
-                           __byte_perm(at(4), at(5), sel), __byte_perm(at(6), at(7), sel));
-          }
-        } else {
-          // nibbles to pairs (dim d, dim d + 4) per key, then to pairs of keys
-          uint32_t o[8][4];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) values(x.v[i], half_scale(x.vs[i], kTinyV, kBigV), o[i]);
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const unsigned sel = d >= 4 ? 0x7632u : 0x5410u;
-            *reinterpret_cast<uint4*>(sv + swz(8 * db + d, kb)) =
-                make_uint4(__byte_perm(o[0][d & 3], o[1][d & 3], sel),
-                           __byte_perm(o[2][d & 3], o[3][d & 3], sel),
-                           __byte_perm(o[4][d & 3], o[5][d & 3], sel),
-                           __byte_perm(o[6][d & 3], o[7][d & 3], sel));
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b.vfull[s]);
-        return true;
-      };
-      // K runs ST - 1 blocks ahead (one group of copies per block, empty past
-      // the end), V two
-      auto ahead = [&](int j) {
-        bool fine = true;
-        if constexpr (BITS == 16) {
-          if (j < blocks) fine = copy_k(j);
-          asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        return fine;
-      };
-      Block<BITS> x, y;
-      bool fine = true;
-      if (blocks > 0) load(x, block_pos(0));
-      for (int j = 0; j < ST - 1 && fine; ++j) fine = ahead(j);
-      for (int j = 0; j < blocks && fine; j += 2) {
-        if (j + 1 < blocks) load(y, block_pos(j + 1));
-        fine = ahead(j + ST - 1) && store(x, j);
-        if (!fine || j + 1 >= blocks) break;
-        if (j + 2 < blocks) load(x, block_pos(j + 2));
-        fine = ahead(j + ST) && store(y, j + 1);
-      }
-      if constexpr (BITS == 16) asm volatile("cp.async.wait_all;" ::: "memory");
-      if (seen) atomicOr(&s_seen, seen);
-    } else {
-      // ---- softmax: thread = matrix row
-      const int m = threadIdx.x, rr = m / heads;
-      const int pos = rr < n ? pos0 + rr : -1;
-      const uint32_t quad = (uint32_t)(warp * 32) << 16;
-      // (a scale of 0 stays a positive factor: -inf * 0 is not a number)
-      const float f = fmaxf(fabsf(a.scale) * kLog2e * q_scale, 1.2e-38f);
-      float top = -INFINITY, sum = 0.f;  // top: in units of log2, of scaled scores
-      // lanes 0-3: the pages of the next block's quarters
-      auto quarter = [&](int j) {
-        const int p = block_pos(j) + 16 * lane;
-        return lane < 4 && j < blocks && p <= last ? kv_page(c, seq, p >> c.g.shift) : -1;
-      };
-      int page = quarter(0);
-      for (int j = 0; j < blocks; ++j) {
-        const int g = base + j;
-        const int p0 = block_pos(j);
-        float x[kKeys];
-        const unsigned present = __ballot_sync(0xffffffffu, page >= 0) & 15u;
-        page = quarter(j + 1);
-        if (!wait_warp(&b.sfull[g & 1], g >> 1)) break;
-        tc_fence_after();
-        tmem_ld32(tm_s + quad + (g & 1) * kKeys, x);
-        tmem_ld32(tm_s + quad + (g & 1) * kKeys + 32, x + 32);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b.sempty[g & 1]);
-        if (!whole(p0) || present != 15) {
-          const int hi = pos - p0;
-          const int lo = a.window ? hi - a.window : -1;  // seen: lo < i <= hi, or i < sinks - p0
-          const int si = a.sinks - p0;
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i) {
-            const bool v = i <= hi && (a.window == 0 || i > lo || i < si) && ((present >> (i >> 4)) & 1);
-            if (!v) x[i] = -INFINITY;
-          }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < kKeys; ++i) mx = fmaxf(mx, x[i]);
-        const float bt = mx * f;
-        // the first scores set the maximum; later it moves when exceeded by 2^8
-        const bool raise = bt > top + 8.f || (top == -INFINITY && bt > -INFINITY);
-        float corr = 1.f;
-        if (raise) {
-          corr = exp2_fast(top - bt);
-          top = bt;
-          sum *= corr;
-        }
-        const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i) x[i] = exp2_fast(fmaf(x[i], f, -ref));
-        float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i) s4[i & 3] += x[i];
-        sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-        // the products of the block before are done: P and O may change
-        if (!wait_warp(&b.pempty, g + 1)) break;
-        tc_fence_after();
-        if (j > 0 && __any_sync(0xffffffffu, raise)) {
-          float o[32];
-#pragma unroll 1
-          for (int k = 0; k < kKvDim; k += 32) {
-            tmem_ld32(tm_o + quad + k, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= corr;
-            tmem_st32(tm_o + quad + k, o);
-          }
-          tmem_st_wait();
-        }
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[8 * ch + i];
-          uint4 w[PP];
-          split8<BITS, PP>(y, w);
-#pragma unroll
-          for (int p = 0; p < PP; ++p)
-            *reinterpret_cast<uint4*>(sp + p * (kRowsM * 128) + swz(m, ch)) = w[p];
-        }
-        tc_fence_before();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b.pfull);
-      }
-      // the matrix products are waited for even after an error: neither TMEM nor
-      // shared memory may go while they run
-      wait_warp(&b.done, dones);
+      const unsigned present = (__ballot_sync(0xffffffffu, held >= 0) >> (4 * (j & 7))) & 15u;
+      if (!wait(&b.sfull[g & 1], g >> 1)) break;
       tc_fence_after();
-      const float il = sum == 0.f ? 0.f : 1.0f / sum;
-      const long long off = (long long)(row0 + rr) * a.out.row +
-                            (long long)(qh0 + m - rr * heads) * a.out.head;
-#pragma unroll 1
-      for (int k = 0; k < kKvDim; k += 32) {
-        float o[32];
-        if (blocks) {
-          tmem_ld32(tm_o + quad + k, o);
-          tmem_ld_wait();
-        }
-        if (rr >= n) continue;
-        const bool none = blocks == 0 || sum == 0.f;
+      tmem_ld32(tm_s + quad + (g & 1) * kKeys, x);
+      tmem_ld32(tm_s + quad + (g & 1) * kKeys + 32, x + 32);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.sempty[g & 1]);
+      if (!w.whole(p0) || present != 15) {
+        // bit i: this row sees position p0 + i
+        auto below = [](int n) {  // the n lowest bits
+          return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
+        };
+        unsigned long long v = below(pos - p0 + 1);
+        if (a.window) v &= ~below(pos - p0 - a.window + 1) | below(a.sinks - p0);
+        const unsigned lo16 = (present & 1 ? 0xffffu : 0u) | (present & 2 ? 0xffff0000u : 0u);
+        const unsigned hi16 = (present & 4 ? 0xffffu : 0u) | (present & 8 ? 0xffff0000u : 0u);
+        const unsigned v0 = (unsigned)v & lo16, v1 = (unsigned)(v >> 32) & hi16;
 #pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          kv_store4(a.out.p, off + k + i, a.type,
-                    none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                         : make_float4(o[i] * il, o[i + 1] * il, o[i + 2] * il, o[i + 3] * il));
+        for (int i = 0; i < 32; ++i) {
+          if (!(v0 & (1u << i))) x[i] = -INFINITY;
+          if (!(v1 & (1u << i))) x[32 + i] = -INFINITY;
+        }
+      }
+      float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int i = 4; i < kKeys; ++i) m4[i & 3] = fmaxf(m4[i & 3], x[i]);
+      const float bt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+      // the first scores set the maximum; later it moves when exceeded by 2^8
+      const bool raise = bt > top + 8.f || (top == -INFINITY && bt > -INFINITY);
+      float corr = 1.f;
+      if (raise) {
+        corr = exp2_fast(top - bt);
+        top = bt;
+        sum *= corr;
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) x[i] = exp2_fast(fmaf(x[i], f, -ref));
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) s4[i & 3] += x[i];
+      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      // this group's products before are done: its P and O may change
+      if (!wait(&b.pempty[g % NG], g / NG + 1)) break;
+      tc_fence_after();
+      if (j >= NG && __any_sync(0xffffffffu, raise)) {
+        float o[32];
+#pragma unroll 1
+        for (int k = 0; k < kKvDim; k += 32) {
+          tmem_ld32(tm_o + (g % NG) * kKvDim + quad + k, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= corr;
+          tmem_st32(tm_o + (g % NG) * kKvDim + quad + k, o);
+        }
+        tmem_st_wait();
+      }
+      uint8_t* pb = sp + (g % NG) * Fm::p_bytes;
+#pragma unroll
+      for (int ch = 0; ch < 8; ++ch) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[8 * ch + i];
+        uint4 o[PP];
+        split8<Fm::pv16, PP>(y, o);
+#pragma unroll
+        for (int p = 0; p < PP; ++p)
+          *reinterpret_cast<uint4*>(pb + p * (kRowsM * 128) + swz(m, ch)) = o[p];
       }
       tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.pfull[g % NG]);
     }
-    base += blocks;
+    // The groups' statistics meet; each then writes half of the dims. The matrix
+    // products are waited for even after an error: neither TMEM nor shared
+    // memory may go while they run.
+    s_top[wg][m] = top;
+    s_sum[wg][m] = sum;
+    wait(&b.done, dones);
+    tc_fence_after();
+    bar<1, 2 * kGroup>();
+    const float t0 = s_top[0][m], t1 = s_top[1][m];
+    const float both = fmaxf(t0, t1), ref = both == -INFINITY ? 0.f : both;
+    const float e0 = exp2_fast(t0 - ref), e1 = exp2_fast(t1 - ref);
+    const float l = e0 * s_sum[0][m] + e1 * s_sum[1][m];
+    const float il = l == 0.f ? 0.f : 1.0f / l;
+    const float w0 = e0 * il, w1 = e1 * il;
+    // the O of a group that had no block in this tile was never written
+    const int g0 = base % NG;  // the group of block 0
+    const bool has0 = w.blocks > (g0 == 0 ? 0 : 1), has1 = NG == 2 && w.blocks > (g0 == 1 ? 0 : 1);
+    const long long off = (long long)(w.row0 + rr) * a.out.row + (long long)(qh0 + hh) * a.out.head;
+#pragma unroll 1
+    for (int k = 64 * wg; k < 64 * wg + 64; k += 32) {
+      float o[32], u[32];
+      if (has0) tmem_ld32(tm_o + quad + k, o);
+      if (has1) tmem_ld32(tm_o + kKvDim + quad + k, u);
+      tmem_ld_wait();
+      if (rr >= w.n) continue;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = (has0 ? o[i] * w0 : 0.f) + (has1 ? u[i] * w1 : 0.f);
+#pragma unroll
+      for (int i = 0; i < 32; i += 4)
+        kv_store4(a.out.p, off + k + i, a.type,
+                  l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                           : make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+    }
+    tc_fence_before();
+    base += w.blocks;
     ++dones;
-    __syncthreads();
+    bar<0, kTileThreads>();
     if (s_dead) break;
-    if (row_by_row(s_seen)) {
-      for (int m = warp; m < n * heads; m += kTileThreads / 32) {
-        const int rr = m / heads;
-        if (pos0 + rr >= 0) kv_attend_row(c, a, seq, pos0 + rr, row0 + rr, qh0 + m - rr * heads);
+    const int seen = s_seen;
+    bar<1, 2 * kGroup>();
+    if (threadIdx.x == 0) s_seen = 0;  // before the next tile's first bar 0
+    if (row_by_row(seen))
+      for (int i = warp; i < w.n * heads; i += 8) {
+        const int ri = i / heads;
+        if (w.pos0 + ri >= 0) kv_attend_row(c, a, seq, w.pos0 + ri, w.row0 + ri, qh0 + i - ri * heads);
       }
-      __syncthreads();
-    }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && s_dead) kv_status(c, kKvTimeout);
-  if (warp == kMmaWarp) tmem_free(s_tmem, 256);
+  bar<0, kTileThreads>();
 }
 
 template <int BITS, bool F32>

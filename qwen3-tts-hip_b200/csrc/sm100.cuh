@@ -45,6 +45,17 @@ __device__ __forceinline__ bool mbar_wait_ns(uint64_t* b, unsigned parity,
     if (t - t0 > limit_ns) return false;
   }
 }
+// The same bound in SM clock cycles: reading %globaltimer costs microseconds,
+// and a wait that is about to be served should not pay for it.
+__device__ __forceinline__ bool mbar_wait_cycles(uint64_t* b, unsigned parity, long long limit) {
+  if (mbar_try(b, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(b, parity)) return true;
+    if (clock64() - t0 > limit) return false;
+  }
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
@@ -126,6 +137,15 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- tcgen05 ----
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -158,6 +178,21 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(const void* p) {
   d |= (uint64_t)2 << 61;                 // layout: 128-byte swizzle
   return d;
 }
+// Shared-memory matrix descriptor of a transposed operand in the 128-byte
+// swizzle: rows of 64 bf16 along the operand's M or N, 8-row groups (8 steps of
+// K) 1024 B apart, the next 64 elements of M or N `next` bytes on.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(const void* p, uint32_t next) {
+  const uint64_t addr = smem_u32(p);
+  uint64_t d = 0;
+  d |= (addr >> 4) & 0x3FFFull;
+  d |= (uint64_t)(next >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// B transposed (its rows in shared memory run along K): or-ed into the above.
+constexpr uint32_t kUmmaTransposeB = 1u << 16;
 // The same for fp16 A and B.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
