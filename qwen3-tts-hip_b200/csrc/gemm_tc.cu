@@ -445,6 +445,10 @@ bool make_map(const void* base, uint64_t inner, uint64_t rows, uint64_t pitch_by
 
 bool tc_available() { return encode_fn() != nullptr; }
 
+bool tc_rows_map(const void* base, uint64_t rows, CUtensorMap* out) {
+  return make_map(base, 128, rows, 256, 16, out);
+}
+
 bool tc_weight_map(const __nv_bfloat16* W, int rows, int K, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<const void*, std::pair<long long, CUtensorMap>> cache;

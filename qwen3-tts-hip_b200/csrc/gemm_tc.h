@@ -32,6 +32,9 @@ struct TcPlan {
 bool tc_available();
 // Host: map of a [rows, K] bf16 weight (box 64 x 64 rows). Cached by pointer.
 bool tc_weight_map(const __nv_bfloat16* W, int rows, int K, CUtensorMap* out);
+// Host: map of a [rows, 128] bf16 array in boxes of 64 x 16 rows (rows past the end
+// read as zeros).
+bool tc_rows_map(const void* base, uint64_t rows, CUtensorMap* out);
 size_t tc_workspace_floats(int tokens, int sm_count);
 
 // Whether launch_linear_tc handles this projection.

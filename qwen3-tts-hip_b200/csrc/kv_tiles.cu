@@ -2,21 +2,24 @@
 // (tcgen05, accumulators in TMEM), bound by the matrix products and the
 // exponentials.
 //
-// A CTA serves 128 matrix rows: the query heads of one kv head (innermost) for
-// consecutive rows of one sequence. It walks the visible positions in blocks
-// of 64 (sinks first, then the window): S = Q K^T (128 x 64, two buffers in
-// TMEM), a thread per row turns its 64 scores into weights P with a running
-// maximum and sum, and O += P V (128 x 128, TMEM). Everything between is in
-// shared memory in the 128-byte swizzle; V is the transposed operand, so K and
-// V keep the pages' own order of rows.
+// A matrix row is a (row, query head of one kv head) pair, heads innermost, rows
+// consecutive in one sequence. A CTA walks the positions that its rows see in
+// blocks (sinks first, then the window): S = Q K^T in TMEM, a thread per matrix
+// row turns its scores into weights P with a running maximum and sum, stored
+// over S as the operand of O += P V (TMEM). Q, K and V are in shared memory in
+// the 128-byte swizzle; V is the transposed operand, so K and V keep the
+// pages' own order of rows.
 //
-// Four warpgroups: two of softmax (thread = matrix row = TMEM lane), which
-// take alternate blocks with statistics and an O of their own that are merged
-// at the end, so that one's exponentials hide the other's waits; one that
-// brings blocks from the pages (16 bits: cp.async, blocks ahead; 4 bits:
-// through registers, two blocks in flight, codes become values); one whose
-// first warp issues the matrix instructions. Registers are moved from the last
-// two to the first two.
+// Four warpgroups: two of softmax; one that makes operands of what the pages
+// hold (16 bits: V from bf16 to fp16 in place; 4 bits: codes to values, through
+// registers); one whose first warp issues the matrix instructions and whose
+// second brings 16-bit rows by TMA. Registers are moved from the last two to the
+// first two. bf16 rows: the softmax groups serve 128 matrix rows each, of one
+// block of 128 positions (shared by both: half the reads of the cache and half
+// the work on operands for each product). fp32 rows, whose operands are two or
+// three times as many: both serve the same 128 matrix rows and take alternate
+// blocks of 64 positions, with statistics and an O of their own that are merged
+// at the end. Either way one group's exponentials hide the other's waits.
 //
 // Number forms. 16-bit pages, bf16 rows: Q K^T in bf16 as it is; P in fp16
 // (2^-12) with V in fp16, which holds a bf16 value exactly from 2^-14 to 2^16.
@@ -37,43 +40,47 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "gemm_tc.h"
 #include "kv.cuh"
 #include "sm100.cuh"
 
 namespace qtts {
 namespace {
 
-constexpr int kRowsM = 128;   // matrix rows of a CTA
-constexpr int kKeys = 64;     // positions per block
+constexpr int kRowsM = 128;   // matrix rows of one product
 constexpr int kGroup = 128;   // threads of a warpgroup
 constexpr int kTileThreads = 4 * kGroup;
 constexpr int kMmaWarp = 12;
-// Registers per thread of the warpgroups (128 at launch): they add up to 512.
-constexpr int kRegsSoftmax = 176, kRegsLoad = 112, kRegsMma = 48;
-static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * 128, "registers the block was given");
 constexpr long long kTileWaitCycles = 4000000000ll;  // two seconds at 2 GHz
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int BITS, bool F32>
 struct Form {
-  static constexpr bool qk16 = BITS == 4;           // Q and K in fp16 (else bf16)
+  static constexpr bool qk16 = BITS == 4;             // Q and K in fp16 (else bf16)
   static constexpr bool pv16 = !(BITS == 16 && F32);  // P and V in fp16
-  static constexpr int qp = !F32 ? 1 : BITS == 16 ? 3 : 2;  // parts of Q
-  static constexpr int pp = qp;                             // parts of P
-  // softmax warpgroups at work: shared memory has no room for two P of three parts
-  static constexpr int groups = BITS == 16 && F32 ? 1 : 2;
-  static constexpr int q_bytes = qp * kRowsM * kKvDim * 2;
-  static constexpr int p_bytes = pp * kRowsM * kKeys * 2;
-  static constexpr int kv_bytes = kKeys * kKvDim * 2;          // K or V of one block
-  static constexpr int stages = F32 ? 2 : 4;
-  static constexpr int smem = q_bytes + groups * p_bytes + stages * 2 * kv_bytes + 1024;
+  static constexpr int parts = !F32 ? 1 : BITS == 16 ? 3 : 2;  // of Q and of P
+  static constexpr bool pair = !F32;                  // two products of 128 matrix rows share K and V
+  static constexpr int rows = pair ? 2 * kRowsM : kRowsM;  // matrix rows of a CTA
+  static constexpr int keys = F32 ? 64 : 128;         // positions per block
+  // TMEM columns of a softmax group's S (fp32), over which P is stored (two
+  // values a column and part), and of its O
+  static constexpr int s_cols = parts * keys / 2 > keys ? parts * keys / 2 : keys;
+  static_assert(2 * s_cols + 2 * kKvDim <= 512, "TMEM");
+  static constexpr int q_bytes = parts * kRowsM * kKvDim * 2;  // of one product
+  static constexpr int kv_bytes = keys * kKvDim * 2;  // K or V of one block
+  static constexpr int stages = F32 ? 3 : 2;  // of K, and of V
+  // Registers per thread of the warpgroups (128 at launch)
+  static constexpr int r_softmax = BITS == 16 ? 200 : 184, r_load = BITS == 16 ? 72 : 104, r_mma = 40;
+  static_assert(2 * r_softmax + r_load + r_mma <= 4 * 128, "registers the block was given");
+  static constexpr int smem = rows / kRowsM * q_bytes + 2 * stages * kv_bytes + 1024;
   static_assert(smem + 2304 <= 227 * 1024, "shared memory of one SM");
 };
 
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 3;
 struct Bars {
-  uint64_t kfull[kMaxStages], kempty[kMaxStages], vfull[kMaxStages], vempty[kMaxStages];
-  uint64_t sfull[2], sempty[2], pfull[2], pempty[2], done;
+  uint64_t kfull[kMaxStages], kempty[kMaxStages], vraw[kMaxStages], vfull[kMaxStages],
+      vempty[kMaxStages];
+  uint64_t sfull[2], pfull[2], done;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -91,7 +98,7 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-// Byte of 16-byte chunk `ch` (0..7) of row `r` in a [rows][64] swizzled tile.
+// Byte of 16-byte chunk `ch` (0..7) of row `r` in a swizzled tile of 64 columns.
 __device__ __forceinline__ int swz(int r, int ch) { return r * 128 + ((ch ^ (r & 7)) << 4); }
 
 // Eight values as `PARTS` operands of 16 bits, each what the ones before left.
@@ -162,7 +169,7 @@ __device__ __forceinline__ bool group_rows(const KvArgs& c, const KvRows& r, int
   return true;
 }
 
-// 4 bits: one block of 64 positions in a loader thread's registers. K and V:
+// 4 bits: 64 positions of a block in a loader thread's registers. K and V:
 // row krow + 8 i, the word of dims 8 kch .. and (bf16, low half) its scale.
 struct Codes {
   uint32_t k[8], ks[8], v[8], vs[8];
@@ -181,7 +188,10 @@ __device__ __forceinline__ void bar() {
 }
 
 // The row tiles of one CTA, the same for every role.
+template <int KEYS>
 struct Walk {
+  static constexpr int kPieces = KEYS / 16;        // a page is at least one piece
+  static constexpr int kHeld = 32 / kPieces;       // blocks whose pages a warp holds
   int begin, end, len, rows_per, window, sinks;
   int row0, n, pos0, last, ns, ws, blocks;
 
@@ -190,38 +200,42 @@ struct Walk {
     n = min(rows_per, end - row0);
     pos0 = len - (end - row0);              // position of the tile's first row
     last = len < 0 ? -1 : pos0 + n - 1;     // < 0: no row holds a position
-    // blocks that some row sees: [0, ns) and [ws, last / 64]
+    // blocks that some row sees: [0, ns) and [ws, last / KEYS]
     const KvSpan lo = kv_span(max(pos0, 0), window, sinks), hi = kv_span(max(last, 0), window, sinks);
-    ns = (hi.sink_end + kKeys - 1) / kKeys;
-    ws = max(lo.first / kKeys, ns);
-    blocks = last < 0 ? 0 : ns + max(0, last / kKeys - ws + 1);
+    ns = (hi.sink_end + KEYS - 1) / KEYS;
+    ws = max(lo.first / KEYS, ns);
+    blocks = last < 0 ? 0 : ns + max(0, last / KEYS - ws + 1);
   }
-  __device__ __forceinline__ int block_pos(int j) const { return (j < ns ? j : j - ns + ws) * kKeys; }
+  __device__ __forceinline__ int block_pos(int j) const { return (j < ns ? j : j - ns + ws) * KEYS; }
   // every row sees every position of the block at p0
   __device__ __forceinline__ bool whole(int p0) const {
-    return pos0 >= 0 && p0 + kKeys - 1 <= pos0 &&
-           (window == 0 || p0 > last - window || p0 + kKeys <= sinks);
+    return pos0 >= 0 && p0 + KEYS - 1 <= pos0 &&
+           (window == 0 || p0 > last - window || p0 + KEYS <= sinks);
   }
-  // Pages of the quarters of eight blocks, one per lane (a page is at least a
-  // quarter), read together when the first of them is wanted.
+  // Pages of the pieces of kHeld blocks, one per lane, read together when the
+  // first of them is wanted.
   __device__ __forceinline__ void refill(const KvArgs& c, int seq, int j, int& held) const {
-    const int lane = threadIdx.x & 31, jj = (j & ~7) + (lane >> 2);
-    const int p = block_pos(jj) + 16 * (lane & 3);
+    const int lane = threadIdx.x & 31, jj = j / kHeld * kHeld + lane / kPieces;
+    const int p = block_pos(jj) + 16 * (lane % kPieces);
     held = jj < blocks && p <= last ? kv_page(c, seq, p >> c.g.shift) : -1;
+  }
+  __device__ __forceinline__ static int held_lane(int j, int piece) {
+    return j % kHeld * kPieces + piece;
   }
 };
 
 template <int BITS, bool F32>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    k_kv_tiles(KvArgs c, KvRows r, KvAttend a, int chunks, int gheads, int rows_per, int tiles) {
+    k_kv_tiles(const __grid_constant__ CUtensorMap map, KvArgs c, KvRows r, KvAttend a, int chunks,
+               int gheads, int rows_per, int tiles) {
   using Fm = Form<BITS, F32>;
-  constexpr int QP = Fm::qp, PP = Fm::pp, ST = Fm::stages, NG = Fm::groups;
+  constexpr int PARTS = Fm::parts, KEYS = Fm::keys, ST = Fm::stages;
   extern __shared__ uint8_t tile_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(tile_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
-  uint8_t* sp = sq + Fm::q_bytes;                 // NG buffers
-  uint8_t* skv = sp + NG * Fm::p_bytes;           // stage s: K at 2 s, V at 2 s + 1 (kv_bytes each)
+  uint8_t* sk = sq + Fm::rows / kRowsM * Fm::q_bytes;  // stages of K, then of V
+  uint8_t* sv = sk + ST * Fm::kv_bytes;
   __shared__ Bars b;
   __shared__ uint32_t s_tmem;
   __shared__ int s_seen;  // what the loaders met (kOdd ..)
@@ -235,7 +249,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int per_head = a.q_heads / c.g.kv_heads;
   const int heads = min(gheads, per_head - chunk * gheads);
   const int qh0 = head * per_head + chunk * gheads;
-  Walk w;
+  Walk<KEYS> w;
   int seq;
   if (!group_rows(c, r, group, &seq, &w.begin, &w.end, &w.len)) return;
   if (a.halt && __ldcg(a.halt + (long long)group * a.halt_stride)) return;
@@ -248,17 +262,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto more = [&](int t) { return (long long)t * rows_per < w.end - w.begin; };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&b.kfull[i], kGroup / 32);
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(&b.kfull[i], BITS == 16 ? 1 : kGroup / 32);
+      mbar_init(&b.vraw[i], 1);
       mbar_init(&b.vfull[i], kGroup / 32);
       mbar_init(&b.kempty[i], 1);
       mbar_init(&b.vempty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.sfull[i], 1);
-      mbar_init(&b.sempty[i], 4);
-      mbar_init(&b.pfull[i], 4);
-      mbar_init(&b.pempty[i], 1);
+      mbar_init(&b.pfull[i], kGroup / 32);
     }
     mbar_init(&b.done, 1);
     fence_mbar_init();
@@ -272,7 +285,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // Dependents may start once every CTA holds its TMEM: one that took columns
   // first and then waited for this grid would never let it finish.
   pdl_trigger();
-  const uint32_t tm_s = s_tmem, tm_o = s_tmem + 2 * kKeys;  // O of group w at + 128 w
+  const uint32_t tm_s = s_tmem, tm_o = s_tmem + 2 * Fm::s_cols;  // group g: + s_cols g, + 128 g
 
   // Bounded waits of a warp: all lanes give up together.
   auto wait = [&](uint64_t* bar, unsigned parity) {
@@ -288,57 +301,109 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp >= kMmaWarp) {
     // ---- matrix instructions: the warp walks together (its operands stay in
     // uniform registers), one lane issues
-    set_registers<kRegsMma, false>();
-    constexpr uint32_t is = Fm::qk16 ? umma_idesc_f16(kRowsM, kKeys) : umma_idesc_bf16(kRowsM, kKeys);
+    set_registers<Fm::r_mma, false>();
+    constexpr uint32_t is = Fm::qk16 ? umma_idesc_f16(kRowsM, KEYS) : umma_idesc_bf16(kRowsM, KEYS);
     constexpr uint32_t io = (Fm::pv16 ? umma_idesc_f16(kRowsM, kKvDim) : umma_idesc_bf16(kRowsM, kKvDim)) |
                             kUmmaTransposeB;
-    const uint64_t dq = umma_desc_sw128(sq), dp = umma_desc_sw128(sp), dkv = umma_desc_sw128(skv),
-                   dvt = umma_desc_sw128_mn(skv, kKeys * 128);
+    const uint64_t dq = umma_desc_sw128(sq), dk = umma_desc_sw128(sk),
+                   dv = umma_desc_sw128_mn(sv, KEYS * 128);
     for (int t = tile0; more(t); t += tiles) {
       w.tile(t);
       bar<0, kTileThreads>();
       if (warp == kMmaWarp) {
-        auto scores = [&](int j) {
+        // S goes to the columns of its softmax group, which held P of the block
+        // before: its product was issued before, and products run in order
+        auto scores = [&](int wg, int j) {
           const int g = base + j, s = g % ST;
-          if (!wait(&b.kfull[s], g / ST) || !wait(&b.sempty[g & 1], (g >> 1) + 1)) return false;
+          if (!wait(&b.kfull[s], g / ST)) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int p = 0; p < QP; ++p)
+            for (int p = 0; p < PARTS; ++p)
 #pragma unroll
               for (int k = 0; k < 8; ++k)  // halves of 64 dims, four steps of 32 bytes in each
-                umma_bf16(tm_s + (g & 1) * kKeys,
-                          dq + (((2 * p + (k >> 2)) * (kRowsM * 128)) >> 4) + 2 * (k & 3),
-                          dkv + ((2 * s * Fm::kv_bytes + (k >> 2) * (kKeys * 128)) >> 4) + 2 * (k & 3),
-                          is, (p | k) != 0);
-            umma_commit(&b.kempty[s]);
-            umma_commit(&b.sfull[g & 1]);
+                umma_bf16(tm_s + wg * Fm::s_cols,
+                          dq + (((Fm::pair ? wg * Fm::q_bytes : 0) +
+                                 (2 * p + (k >> 2)) * (kRowsM * 128)) >> 4) + 2 * (k & 3),
+                          dk + ((s * Fm::kv_bytes + (k >> 2) * (KEYS * 128)) >> 4) + 2 * (k & 3), is,
+                          (p | k) != 0);
+            if (!Fm::pair || wg == 1) umma_commit(&b.kempty[s]);
+            umma_commit(&b.sfull[wg]);
           }
           __syncwarp();
           return true;
         };
-        bool fine = (w.blocks < 1 || scores(0)) && (w.blocks < 2 || scores(1));
-        for (int j = 0; j < w.blocks && fine; ++j) {
-          const int g = base + j, s = g % ST, wg = g % NG;
-          if (!wait(&b.vfull[s], g / ST) || !wait(&b.pfull[wg], g / NG)) break;
+        // first: nothing to add to; n: how many products of this group came before
+        auto values = [&](int wg, int j, bool first, int n) {
+          const int g = base + j, s = g % ST;
+          if (!wait(&b.vfull[s], g / ST) || !wait(&b.pfull[wg], n)) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int p = 0; p < PP; ++p)
+            for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_bf16(tm_o + wg * kKvDim, dp + ((wg * Fm::p_bytes + p * (kRowsM * 128)) >> 4) + 2 * k,
-                          dvt + (((2 * s + 1) * Fm::kv_bytes + k * 16 * 128) >> 4), io,
-                          j >= NG || (p | k) != 0);
-            umma_commit(&b.vempty[s]);
-            umma_commit(&b.pempty[wg]);
+              for (int k = 0; k < KEYS / 16; ++k)
+                umma_16_ts(tm_o + wg * kKvDim, tm_s + wg * Fm::s_cols + p * (KEYS / 2) + 8 * k,
+                           dv + ((s * Fm::kv_bytes + k * 16 * 128) >> 4), io, !first || (p | k) != 0);
+            if (!Fm::pair || wg == 1) umma_commit(&b.vempty[s]);
           }
           __syncwarp();
-          fine = j + 2 >= w.blocks || scores(j + 2);
+          return true;
+        };
+        bool fine = true;
+        if constexpr (Fm::pair) {
+          fine = w.blocks < 1 || (scores(0, 0) && scores(1, 0));
+          for (int j = 0; j < w.blocks && fine; ++j)
+            for (int wg = 0; wg < 2 && fine; ++wg)
+              fine = values(wg, j, j == 0, base + j) && (j + 1 >= w.blocks || scores(wg, j + 1));
+        } else {
+          fine = (w.blocks < 1 || scores(base & 1, 0)) && (w.blocks < 2 || scores((base + 1) & 1, 1));
+          for (int j = 0; j < w.blocks && fine; ++j)
+            fine = values((base + j) & 1, j, j < 2, (base + j) >> 1) &&
+                   (j + 2 >= w.blocks || scores((base + j) & 1, j + 2));
         }
         // the output is read, and the next tile begun, after every product
         if (elect_one()) umma_commit(&b.done);
         __syncwarp();
+      } else if (BITS == 16 && warp == kMmaWarp + 1) {
+        // ---- 16-bit rows, by TMA: a lane per piece of 16 positions and half of 64
+        // dims; a piece that is not there is read past the map's rows, as zeros
+        const int page_rows = c.g.layers * 2 * c.g.kv_heads << c.g.shift;
+        const int tile_row = (a.layer * 2 * c.g.kv_heads + head) << c.g.shift;
+        const int mask = (1 << c.g.shift) - 1;
+        const int piece = lane % w.kPieces, half = lane / w.kPieces;  // lanes past two halves: none
+        auto page_of = [&](int j) {
+          const int p = w.block_pos(j) + 16 * piece;
+          return j < w.blocks && p <= w.last ? kv_page(c, seq, p >> c.g.shift) : -1;
+        };
+        int page = page_of(0);
+        bool fine = true;
+        int j = 0;
+        for (; j < w.blocks; ++j) {
+          const int g = base + j, s = g % ST, p = w.block_pos(j) + 16 * piece;
+          const int row = page >= 0 ? page * page_rows + tile_row + (p & mask) : 0x7ffffff0;
+          page = page_of(j + 1);  // in flight during the copies
+          const int to = s * Fm::kv_bytes + half * (KEYS * 128) + piece * 2048;
+          if (!(fine = wait(&b.kempty[s], g / ST + 1))) break;
+          if (lane == 0) mbar_expect_tx(&b.kfull[s], Fm::kv_bytes);
+          __syncwarp();
+          if (half < 2) tma_load_2d(sk + to, &map, 64 * half, row, &b.kfull[s]);
+          if (!(fine = wait(&b.vempty[s], g / ST + 1))) {
+            ++j;  // K of this block is on its way
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(&b.vraw[s], Fm::kv_bytes);
+          __syncwarp();
+          if (half < 2)
+            tma_load_2d(sv + to, &map, 64 * half,
+                        row == 0x7ffffff0 ? row : row + (c.g.kv_heads << c.g.shift), &b.vraw[s]);
+        }
+        // no copy may still be landing when the CTA goes
+        if (!fine)
+          for (int i = max(0, j - ST); i < j; ++i) {
+            wait(&b.kfull[(base + i) % ST], (base + i) / ST);
+            if (i < j - 1) wait(&b.vraw[(base + i) % ST], (base + i) / ST);
+          }
       }
       base += w.blocks;
       bar<0, kTileThreads>();
@@ -356,78 +421,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (warp >= 8) {
     // ---- loaders
-    set_registers<kRegsLoad, false>();
+    set_registers<Fm::r_load, false>();
     const int lt = threadIdx.x - 2 * kGroup;
     const int krow = lt >> 4, kch = lt & 15;      // rows krow + 8 i, dims 8 kch ..
     const long long page_bytes = kv_page_bytes(c.g);
     const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
     const long long v_off = kv_tile_bytes(c.g) * c.g.kv_heads;  // from K's tile to V's
     const int mask = (1 << c.g.shift) - 1;
-    const int at0 = (kch >> 3) * (kKeys * 128) + swz(krow, kch & 7);  // row krow + 8 i: + 1024 i
+    const int at0 = (kch >> 3) * (KEYS * 128) + swz(krow, kch & 7);  // row krow + 8 i: + 1024 i
     for (int t = tile0; more(t); t += tiles) {
       w.tile(t);
       bar<0, kTileThreads>();
       int seen = 0;
       if constexpr (BITS == 16) {
-        // Copies: group a holds K of block a + 1 and V of block a (K first: its
-        // product comes earlier), group -1 K of block 0. They are started ST - 2
-        // groups ahead; positions that are not there become 0.
-        int held[2] = {-1, -1};
-        auto start = [&](int j, int which) {  // block j, 0: K, 1: V
-          if (j >= w.blocks) return true;
+        // V of each block as it lands. Positions past the rows' last become 0 (their
+        // page may hold anything, and NaN * 0 is not 0). pv16: bf16 becomes fp16,
+        // and the largest magnitude says whether it fits; else only NaN or infinity
+        // where some rows look and others do not matters.
+        unsigned top = 0u;  // largest magnitudes, per half word
+        for (int j = 0; j < w.blocks; ++j) {
           const int g = base + j, s = g % ST, p0 = w.block_pos(j);
-          if ((j & 7) == 0) w.refill(c, seq, j, held[which]);
-          if (!wait(which ? &b.vempty[s] : &b.kempty[s], g / ST + 1)) return false;
-          const uint32_t dst = smem_u32(skv + (2 * s + which) * Fm::kv_bytes) + at0;
-          const unsigned char* from = kbase + (which ? v_off : 0) + krow * 256 + kch * 16;
-#pragma unroll
-          for (int qu = 0; qu < 4; ++qu) {
-            const int page = __shfl_sync(0xffffffffu, held[which], 4 * (j & 7) + qu);
-            const int p = p0 + 16 * qu;
-            const unsigned char* src = from + max(page, 0) * page_bytes + (p & mask) * 256;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool ok = page >= 0 && p + krow + 8 * h <= w.last;
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 2048 * qu + 1024 * h),
-                           "l"(src + 2048 * h), "r"(ok ? 16 : 0)
-                           : "memory");
-            }
-          }
-          return true;
-        };
-        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-        auto give = [&](uint64_t* full) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full);
-        };
-        unsigned top = 0u;  // largest magnitudes of V, per half word
-        bool fine = start(0, 0);
-        commit();
-        for (int i = 0; i < ST - 2 && fine; ++i) {
-          fine = start(i + 1, 0) && start(i, 1);
-          commit();
-        }
-        if (fine && w.blocks > 0) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-          give(&b.kfull[base % ST]);
-        }
-        for (int j = 0; j < w.blocks && fine; ++j) {
-          if constexpr (ST == 2) {  // nothing ahead: started now
-            fine = start(j + 1, 0) && start(j, 1);
-            commit();
-            if (!fine) break;
-          }
-          asm volatile("cp.async.wait_group %0;" ::"n"(ST >= 3 ? ST - 3 : 0) : "memory");
-          if (j + 1 < w.blocks) give(&b.kfull[(base + j + 1) % ST]);
-          const int s = (base + j) % ST;
-          uint8_t* sv = skv + (2 * s + 1) * Fm::kv_bytes + at0;
-          // pv16: bf16 becomes fp16, and the largest magnitude says whether it fits;
-          // else only NaN or infinity where some rows look and others do not matters
-          if (Fm::pv16 || !w.whole(w.block_pos(j))) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint4 v = *reinterpret_cast<const uint4*>(sv + 1024 * i);
+          if (!wait(&b.vraw[s], g / ST)) break;
+          uint8_t* at = sv + s * Fm::kv_bytes + at0;
+          const bool whole = w.whole(p0);
+          if (Fm::pv16 || !whole) {
+#pragma unroll 8
+            for (int i = 0; i < KEYS / 8; ++i) {
+              uint4 v = *reinterpret_cast<const uint4*>(at + 1024 * i);
+              if (!whole && p0 + krow + 8 * i > w.last) v = make_uint4(0u, 0u, 0u, 0u);
               top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
                                            __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
               if constexpr (Fm::pv16) {
@@ -435,32 +456,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 v.y = pack_pair<true>(bf16lo(v.y), bf16hi(v.y));
                 v.z = pack_pair<true>(bf16lo(v.z), bf16hi(v.z));
                 v.w = pack_pair<true>(bf16lo(v.w), bf16hi(v.w));
-                *reinterpret_cast<uint4*>(sv + 1024 * i) = v;
               }
+              *reinterpret_cast<uint4*>(at + 1024 * i) = v;
             }
           }
-          give(&b.vfull[s]);
-          if constexpr (ST > 2) {
-            fine = start(j + ST - 1, 0) && start(j + ST - 2, 1);
-            commit();
-          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.vfull[s]);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
         const unsigned m = max(top & 0xffffu, top >> 16);
         // bf16 bits: 0x7f80 infinity; fp16 ends below 2^16 (0x4780); 2^-11 is 0x3a00
         seen = m >= (Fm::pv16 ? 0x4780u : 0x7f80u) ? kOdd : 0;
         if (Fm::pv16) seen |= (m ? kAnyV : 0) | (m >= 0x3a00u ? kBigV : 0);
       } else {
         int held = -1;
-        auto load = [&](Codes& x, int j) {
-          const int p0 = w.block_pos(j);
-          if ((j & 7) == 0) w.refill(c, seq, j, held);
+        constexpr int U = KEYS / 64;  // units of 64 positions per block
+        auto load = [&](Codes& x, int u) {
+          const int j = u / U, pc0 = 4 * (u % U), p0 = w.block_pos(j);
+          if (u % (U * w.kHeld) == 0) w.refill(c, seq, j, held);
           const unsigned char* from = kbase + krow * 64 + kv_code_word_at(8 * kch);
           const unsigned char* from_s = kbase + (kKvCodeBytes << c.g.shift) + krow * 8 + 2 * (kch >> 2);
 #pragma unroll
           for (int qu = 0; qu < 4; ++qu) {
-            const int page = __shfl_sync(0xffffffffu, held, 4 * (j & 7) + qu);
-            const int p = p0 + 16 * qu;
+            const int page = __shfl_sync(0xffffffffu, held, w.held_lane(j, pc0 + qu));
+            const int p = p0 + 16 * (pc0 + qu);
             const long long at = max(page, 0) * page_bytes;
             const unsigned char* src = from + at + (p & mask) * 64;
             const unsigned char* src_s = from_s + at + (p & mask) * 8;
@@ -493,31 +512,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
                          __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
         };
-        auto store = [&](const Codes& x, int j) {
-          const int g = base + j, s = g % ST;
-          uint8_t* sk = skv + 2 * s * Fm::kv_bytes + at0;
-          if (!wait(&b.kempty[s], g / ST + 1)) return false;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) put(sk + 1024 * i, x.k[i], x.ks[i], kAnyK, kBigK);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b.kfull[s]);
-          if (!wait(&b.vempty[s], g / ST + 1)) return false;
+        auto store = [&](const Codes& x, int u) {
+          const int g = base + u / U, s = g % ST;
+          const int at = at0 + u % U * (64 * 128);
+          const bool opens = u % U == 0, closes = u % U == U - 1;
+          if (opens && !wait(&b.kempty[s], g / ST + 1)) return false;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            put(sk + Fm::kv_bytes + 1024 * i, x.v[i], x.vs[i], kAnyV, kBigV);
+            put(sk + s * Fm::kv_bytes + at + 1024 * i, x.k[i], x.ks[i], kAnyK, kBigK);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(&b.vfull[s]);
+          if (closes && lane == 0) mbar_arrive(&b.kfull[s]);
+          if (opens && !wait(&b.vempty[s], g / ST + 1)) return false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            put(sv + s * Fm::kv_bytes + at + 1024 * i, x.v[i], x.vs[i], kAnyV, kBigV);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (closes && lane == 0) mbar_arrive(&b.vfull[s]);
           return true;
         };
+        const int units = w.blocks * U;
         Codes x, y;
-        if (w.blocks > 0) load(x, 0);
-        for (int j = 0; j < w.blocks; j += 2) {
-          if (j + 1 < w.blocks) load(y, j + 1);
-          if (!store(x, j) || j + 1 >= w.blocks) break;
-          if (j + 2 < w.blocks) load(x, j + 2);
-          if (!store(y, j + 1)) break;
+        if (units > 0) load(x, 0);
+        for (int u = 0; u < units; u += 2) {
+          if (u + 1 < units) load(y, u + 1);
+          if (!store(x, u) || u + 1 >= units) break;
+          if (u + 2 < units) load(x, u + 2);
+          if (!store(y, u + 1)) break;
         }
       }
       if (seen) atomicOr(&s_seen, seen);
@@ -530,16 +552,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 
   // ---- softmax: thread = matrix row
-  set_registers<kRegsSoftmax, true>();
+  set_registers<Fm::r_softmax, true>();
   const int wg = warp >> 2, m = threadIdx.x & (kGroup - 1);
-  const int rr = m / heads, hh = m - rr * heads;
+  const int mi = Fm::pair ? wg * kRowsM + m : m;  // matrix row of the CTA
+  const int rr = mi / heads, hh = mi - rr * heads;
   const uint32_t quad = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
   unsigned dones = 0;
   for (int t = tile0; more(t); t += tiles) {
     w.tile(t);
     float q_scale = 1.f;  // what undoes the row's power of two
     {
-      // Q: with two groups each stores half of the dims of its row
+      // Q of this thread's row (two threads on one row: half of the dims each)
       const bool in = rr < w.n;
       const long long off = (long long)(w.row0 + rr) * a.q.row + (long long)(qh0 + hh) * a.q.head;
       float up = 1.f;
@@ -561,7 +584,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // a negative scale goes into Q, so that masked scores are -inf either way
       if (a.scale < 0.f) up = -up;
 #pragma unroll 4
-      for (int ch = 8 * wg; ch < 8 * wg + 8; ++ch) {
+      for (int ch = Fm::pair ? 0 : 8 * wg; ch < (Fm::pair ? 16 : 8 * wg + 8); ++ch) {
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (in) {
           const float4 y = kv_load4(a.q.p, off + 8 * ch, a.type);
@@ -569,11 +592,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           x[0] = y.x * up; x[1] = y.y * up; x[2] = y.z * up; x[3] = y.w * up;
           x[4] = z.x * up; x[5] = z.y * up; x[6] = z.z * up; x[7] = z.w * up;
         }
-        uint4 o[QP];
-        split8<Fm::qk16, QP>(x, o);
+        uint4 o[PARTS];
+        split8<Fm::qk16, PARTS>(x, o);
 #pragma unroll
-        for (int p = 0; p < QP; ++p)
-          *reinterpret_cast<uint4*>(sq + (2 * p + (ch >> 3)) * (kRowsM * 128) + swz(m, ch & 7)) = o[p];
+        for (int p = 0; p < PARTS; ++p)
+          *reinterpret_cast<uint4*>(sq + (Fm::pair ? wg * Fm::q_bytes : 0) +
+                                    (2 * p + (ch >> 3)) * (kRowsM * 128) + swz(m, ch & 7)) = o[p];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -583,44 +607,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const float f = fmaxf(fabsf(a.scale) * kLog2e * q_scale, 1.2e-38f);
     float top = -INFINITY, sum = 0.f;  // top: in units of log2, of scaled scores
     int held = -1, held_at = -1;
-    int first = NG == 1 ? 0 : (wg - base) & 1;  // this group's blocks: (base + j) % 2 == wg
-    if (wg >= NG) first = w.blocks;
-    for (int j = first; j < w.blocks; j += NG) {
+    const uint32_t my_s = tm_s + quad + wg * Fm::s_cols, my_o = tm_o + quad + wg * kKvDim;
+    // this group's blocks: all, or those with (base + j) % 2 == wg
+    for (int j = Fm::pair ? 0 : (wg - base) & 1; j < w.blocks; j += Fm::pair ? 1 : 2) {
       const int g = base + j;
       const int p0 = w.block_pos(j);
-      float x[kKeys];
-      if ((j >> 3) != held_at) {
-        held_at = j >> 3;
+      float x[KEYS];
+      if (j / w.kHeld != held_at) {
+        held_at = j / w.kHeld;
         w.refill(c, seq, j, held);
       }
-      const unsigned present = (__ballot_sync(0xffffffffu, held >= 0) >> (4 * (j & 7))) & 15u;
-      if (!wait(&b.sfull[g & 1], g >> 1)) break;
+      constexpr unsigned all = (1u << w.kPieces) - 1u;
+      const unsigned present =
+          (__ballot_sync(0xffffffffu, held >= 0) >> w.held_lane(j, 0)) & all;
+      // S is there, and so is everything issued before it: this group's P and O
+      // of the blocks before may change
+      if (!wait(&b.sfull[wg], Fm::pair ? g : g >> 1)) break;
       tc_fence_after();
-      tmem_ld32(tm_s + quad + (g & 1) * kKeys, x);
-      tmem_ld32(tm_s + quad + (g & 1) * kKeys + 32, x + 32);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b.sempty[g & 1]);
-      if (!w.whole(p0) || present != 15) {
-        // bit i: this row sees position p0 + i
-        auto below = [](int n) {  // the n lowest bits
-          return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
-        };
-        unsigned long long v = below(pos - p0 + 1);
-        if (a.window) v &= ~below(pos - p0 - a.window + 1) | below(a.sinks - p0);
-        const unsigned lo16 = (present & 1 ? 0xffffu : 0u) | (present & 2 ? 0xffff0000u : 0u);
-        const unsigned hi16 = (present & 4 ? 0xffffu : 0u) | (present & 8 ? 0xffff0000u : 0u);
-        const unsigned v0 = (unsigned)v & lo16, v1 = (unsigned)(v >> 32) & hi16;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!(v0 & (1u << i))) x[i] = -INFINITY;
-          if (!(v1 & (1u << i))) x[32 + i] = -INFINITY;
+      for (int i = 0; i < KEYS; i += 32) tmem_ld32(my_s + i, x + i);
+      tmem_ld_wait();
+      if (!w.whole(p0) || present != all) {
+        // bits: this row sees position p0 + i
+        const int hi = pos - p0 + 1;                                // i < hi
+        const int lo = a.window ? hi - a.window : 0;                // and i >= lo
+        const int si = a.sinks - p0;                                // or i < si
+        auto below = [](int n) {  // the n lowest bits
+          return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+        };
+#pragma unroll
+        for (int q = 0; q < KEYS / 32; ++q) {
+          unsigned v = below(hi - 32 * q) & (~below(lo - 32 * q) | below(si - 32 * q));
+          v &= ((present >> (2 * q)) & 1 ? 0xffffu : 0u) | ((present >> (2 * q)) & 2 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(v & (1u << i))) x[32 * q + i] = -INFINITY;
         }
       }
       float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < kKeys; ++i) m4[i & 3] = fmaxf(m4[i & 3], x[i]);
+      for (int i = 4; i < KEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], x[i]);
       const float bt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
       // the first scores set the maximum; later it moves when exceeded by 2^8
       const bool raise = bt > top + 8.f || (top == -INFINITY && bt > -INFINITY);
@@ -631,76 +657,102 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sum *= corr;
       }
       const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int i = 0; i < kKeys; ++i) x[i] = exp2_fast(fmaf(x[i], f, -ref));
       float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      // weights, 32 at a time, stored as P over S: per part KEYS / 2 columns of
+      // two values (every score has been read)
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i) s4[i & 3] += x[i];
+      for (int i = 0; i < KEYS; i += 32) {
+#pragma unroll
+        for (int k = i; k < i + 32; ++k) {
+          x[k] = exp2_fast(fmaf(x[k], f, -ref));
+          s4[k & 3] += x[k];
+        }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          uint32_t o[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float& u = x[i + 2 * k];
+            float& v = x[i + 2 * k + 1];
+            if (!Fm::pv16 && p + 1 < PARTS) {
+              // cut, not rounded: one permute, and the next part takes the rest
+              const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
+              o[k] = __byte_perm(ub, vb, 0x7632);
+              u -= __uint_as_float(ub & 0xffff0000u);
+              v -= __uint_as_float(vb & 0xffff0000u);
+            } else {
+              o[k] = pack_pair<Fm::pv16>(u, v);
+              if (p + 1 < PARTS) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&o[k]));
+                u -= h.x;
+                v -= h.y;
+              }
+            }
+          }
+          tmem_st16(my_s + p * (KEYS / 2) + i / 2, o);
+        }
+      }
       sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      // this group's products before are done: its P and O may change
-      if (!wait(&b.pempty[g % NG], g / NG + 1)) break;
-      tc_fence_after();
-      if (j >= NG && __any_sync(0xffffffffu, raise)) {
+      if (j >= (Fm::pair ? 1 : 2) && __any_sync(0xffffffffu, raise)) {
         float o[32];
 #pragma unroll 1
         for (int k = 0; k < kKvDim; k += 32) {
-          tmem_ld32(tm_o + (g % NG) * kKvDim + quad + k, o);
+          tmem_ld32(my_o + k, o);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= corr;
-          tmem_st32(tm_o + (g % NG) * kKvDim + quad + k, o);
+          tmem_st32(my_o + k, o);
         }
-        tmem_st_wait();
       }
-      uint8_t* pb = sp + (g % NG) * Fm::p_bytes;
-#pragma unroll
-      for (int ch = 0; ch < 8; ++ch) {
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[8 * ch + i];
-        uint4 o[PP];
-        split8<Fm::pv16, PP>(y, o);
-#pragma unroll
-        for (int p = 0; p < PP; ++p)
-          *reinterpret_cast<uint4*>(pb + p * (kRowsM * 128) + swz(m, ch)) = o[p];
-      }
+      tmem_st_wait();
       tc_fence_before();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b.pfull[g % NG]);
+      if (lane == 0) mbar_arrive(&b.pfull[wg]);
     }
-    // The groups' statistics meet; each then writes half of the dims. The matrix
-    // products are waited for even after an error: neither TMEM nor shared
-    // memory may go while they run.
-    s_top[wg][m] = top;
-    s_sum[wg][m] = sum;
+    // The matrix products are waited for even after an error: neither TMEM nor
+    // shared memory may go while they run.
     wait(&b.done, dones);
     tc_fence_after();
-    bar<1, 2 * kGroup>();
-    const float t0 = s_top[0][m], t1 = s_top[1][m];
-    const float both = fmaxf(t0, t1), ref = both == -INFINITY ? 0.f : both;
-    const float e0 = exp2_fast(t0 - ref), e1 = exp2_fast(t1 - ref);
-    const float l = e0 * s_sum[0][m] + e1 * s_sum[1][m];
-    const float il = l == 0.f ? 0.f : 1.0f / l;
-    const float w0 = e0 * il, w1 = e1 * il;
-    // the O of a group that had no block in this tile was never written
-    const int g0 = base % NG;  // the group of block 0
-    const bool has0 = w.blocks > (g0 == 0 ? 0 : 1), has1 = NG == 2 && w.blocks > (g0 == 1 ? 0 : 1);
     const long long off = (long long)(w.row0 + rr) * a.out.row + (long long)(qh0 + hh) * a.out.head;
-#pragma unroll 1
-    for (int k = 64 * wg; k < 64 * wg + 64; k += 32) {
-      float o[32], u[32];
-      if (has0) tmem_ld32(tm_o + quad + k, o);
-      if (has1) tmem_ld32(tm_o + kKvDim + quad + k, u);
-      tmem_ld_wait();
-      if (rr >= w.n) continue;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = (has0 ? o[i] * w0 : 0.f) + (has1 ? u[i] * w1 : 0.f);
+    auto put = [&](int k, const float (&o)[32], float by, bool none) {
+      if (rr >= w.n) return;
 #pragma unroll
       for (int i = 0; i < 32; i += 4)
         kv_store4(a.out.p, off + k + i, a.type,
-                  l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                  none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                       : make_float4(o[i] * by, o[i + 1] * by, o[i + 2] * by, o[i + 3] * by));
+    };
+    if constexpr (Fm::pair) {
+#pragma unroll 1
+      for (int k = 0; k < kKvDim; k += 32) {
+        float o[32];
+        if (w.blocks) tmem_ld32(my_o + k, o);
+        tmem_ld_wait();
+        put(k, o, 1.0f / sum, sum == 0.f);
+      }
+    } else {
+      // the groups' statistics meet; each then writes half of the dims
+      s_top[wg][m] = top;
+      s_sum[wg][m] = sum;
+      bar<1, 2 * kGroup>();
+      const float t0 = s_top[0][m], t1 = s_top[1][m];
+      const float both = fmaxf(t0, t1), ref = both == -INFINITY ? 0.f : both;
+      const float e0 = exp2_fast(t0 - ref), e1 = exp2_fast(t1 - ref);
+      const float l = e0 * s_sum[0][m] + e1 * s_sum[1][m];
+      const float il = 1.0f / l;
+      // the O of a group that had no block in this tile was never written
+      const int g0 = base & 1;  // the group of block 0
+      const bool has0 = w.blocks > (g0 == 0 ? 0 : 1), has1 = w.blocks > (g0 == 1 ? 0 : 1);
+#pragma unroll 1
+      for (int k = 64 * wg; k < 64 * wg + 64; k += 32) {
+        float o[32], u[32];
+        if (has0) tmem_ld32(tm_o + quad + k, o);
+        if (has1) tmem_ld32(tm_o + kKvDim + quad + k, u);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = (has0 ? o[i] * e0 : 0.f) + (has1 ? u[i] * e1 : 0.f);
+        put(k, o, il, l == 0.f);
+      }
     }
     tc_fence_before();
     base += w.blocks;
@@ -737,12 +789,15 @@ cudaError_t tiles(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStrea
       ready[dev] = true;
     }
   }
+  CUtensorMap map{};
+  if (BITS == 16 && !tc_rows_map(c.pool, (uint64_t)c.g.pages * kv_page_bytes(c.g) / (2 * kKvDim), &map))
+    return cudaErrorNotSupported;
   const int group = a.q_heads / c.g.kv_heads;
   const int gheads = std::min(group, kRowsM), chunks = (group + gheads - 1) / gheads;
-  const int rows_per = kRowsM / gheads;
+  const int rows_per = Form<BITS, F32>::rows / gheads;
   const int n = (r.max_rows + rows_per - 1) / rows_per;
   return launch(kernel, dim3((unsigned)((long long)n * r.groups), (unsigned)(c.g.kv_heads * chunks)),
-                dim3(kTileThreads), (size_t)smem, stream, c, r, a, chunks, gheads, rows_per, n);
+                dim3(kTileThreads), (size_t)smem, stream, map, c, r, a, chunks, gheads, rows_per, n);
 }
 
 }  // namespace
