@@ -16,13 +16,22 @@
 // Column pairs 2 t, 2 t + 1 of an accumulator sit in one lane: summing the
 // parts costs one addition.
 //
-// 4-bit rows: codes become bf16 integers (exact) by bit operations. K: each
-// group of 32 dims accumulates apart and its scale multiplies the fp32 sum; V:
-// the scale multiplies the fp32 weight before it is split into parts.
+// 4-bit rows: codes become small integers by bit operations, a code's nibble
+// placed in the mantissa of 16. K: each group of 32 dims accumulates apart and
+// its scale multiplies the fp32 sum. V, fp32 rows: the scale multiplies the fp32
+// weight before it is split into parts. V, bf16 rows: code * scale is exact in
+// fp16 (11 bits) for scales of 2^-14 to 2^12, and weights are rounded to fp16
+// (2^-12); a tile with other scales takes the first way.
+//
+// Bound by bytes in flight and by issue. 4-bit tiles (four contiguous pieces,
+// 2,304 bytes) come by bulk copies into a ring of each warp's own, kRing tiles
+// ahead; 16-bit ones into registers, refilled in place: the next K while its
+// weights meet V, the next V while its K is scored.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
 // CTAs of a cluster through distributed shared memory, both in a fixed order.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <mutex>
@@ -34,11 +43,13 @@
 namespace qtts {
 namespace {
 
-constexpr int kStepWarps = 8;
+constexpr int kStepWarps = 4;
 constexpr int kStepThreads = kStepWarps * 32;
 constexpr int kStepHeads = 4;   // query heads of one CTA
+constexpr int kRing = 4;        // 4-bit tiles in flight per warp
 constexpr int kTile = 16;       // positions of one matrix instruction; a page is a multiple
 constexpr int kMaxCluster = 16;
+constexpr long long kStepWaitCycles = 4000000000ll;  // two seconds at 2 GHz
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -52,62 +63,114 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Nibbles i and i + 4 (of the two 16-bit halves: one each) of w as bf16
-// integers n = code - 8: 128 + code is a bf16 with the code in its low bits.
+__device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1, float c0, float c2) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      " {%10,%11,%12,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(0.f), "f"(c2));
+}
+__device__ __forceinline__ void mma16816_half(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      " {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t shifted(uint32_t w, int left) {
+  return left >= 0 ? w << left : w >> -left;
+}
+// Nibble i of each 16-bit half of w as 16 + code: the nibble in the upper
+// mantissa bits of 16.0, bf16 (bits 3-6) or fp16 (bits 6-9).
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, int i) {
+  return (shifted(w, 3 - 4 * i) & 0x00780078u) | 0x41804180u;
+}
+__device__ __forceinline__ uint32_t nibbles_half(uint32_t w, int i) {
+  return (shifted(w, 6 - 4 * i) & 0x03c003c0u) | 0x4c004c00u;
+}
+// The same as n = code - 8, exact.
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
-  const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  const uint32_t u = nibbles_bf16(w, i);
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
-                                   __nv_bfloat162(__float2bfloat16(136.f), __float2bfloat16(136.f)));
+                                   __nv_bfloat162(__float2bfloat16(24.f), __float2bfloat16(24.f)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// What one lane (g = lane / 4, t = lane % 4) loads of a tile.
+// What one lane (g = lane / 4, t = lane % 4) holds of a tile.
 template <int BITS>
-struct Tile;
+struct Keys;
 template <>
-struct Tile<16> {
+struct Keys<16> {
   uint4 k[2][4];  // rows g, g + 8; dims 32 j + 8 t ..
-  uint4 v[4][2];  // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9; dims 8 g .., 64 + 8 g ..
 };
 template <>
-struct Tile<4> {
+struct Keys<4> {
   uint4 k[2];     // rows g, g + 8: word j = dims 32 j + 8 t ..
   uint2 ks[2];    // their four scales
-  uint4 v[4];     // positions as above: word j holds dims 32 j + 8 (g / 2) ..
+};
+template <int BITS>
+struct Values;
+template <>
+struct Values<16> {
+  uint4 v[4][2];  // positions v_pos(t, i); dims 8 g .., 64 + 8 g ..
+};
+template <>
+struct Values<4> {
+  uint4 v[4];     // positions v_pos(t, i): word j holds dims 32 j + 8 (g / 2) ..
   uint2 vs[4];
 };
 
-__device__ __forceinline__ int v_pos(int t, int i) { return 2 * t + (i & 1) + 8 * (i >> 1); }
+// The positions of a lane's V operand (any assignment does, if the weights
+// follow it): consecutive rows for neighbouring t keep the shared-memory reads
+// of a 4-bit tile at two to a bank.
+__device__ __forceinline__ int v_pos(int t, int i) { return t + 4 * i; }
 
-template <int BITS>
-__device__ __forceinline__ void load_tile(Tile<BITS>& x, const unsigned char* kt,
-                                          const unsigned char* vt, int row0, int shift) {
+// A 4-bit tile in shared memory.
+struct __align__(16) Packed {
+  uint4 k[kTile * 4], v[kTile * 4];  // 64 bytes a row
+  uint2 ks[kTile], vs[kTile];
+};
+
+// 16 bits: rows of a K (V) tile from global memory.
+__device__ __forceinline__ void load_keys(Keys<16>& x, const unsigned char* rows) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if constexpr (BITS == 16) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+  for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x.k[r][j] = __ldcg(reinterpret_cast<const uint4*>(kt + (row0 + g + 8 * r) * 256) + 4 * j + t);
+    for (int j = 0; j < 4; ++j)
+      x.k[r][j] = __ldcg(reinterpret_cast<const uint4*>(rows + (g + 8 * r) * 256) + 4 * j + t);
+}
+__device__ __forceinline__ void load_values(Values<16>& x, const unsigned char* rows) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        x.v[i][h] = __ldcg(reinterpret_cast<const uint4*>(vt + (row0 + v_pos(t, i)) * 256) + 8 * h + g);
-  } else {
-    const unsigned char* ks = kt + (kKvCodeBytes << shift);
-    const unsigned char* vs = vt + (kKvCodeBytes << shift);
+    for (int h = 0; h < 2; ++h)
+      x.v[i][h] = __ldcg(reinterpret_cast<const uint4*>(rows + v_pos(t, i) * 256) + 8 * h + g);
+}
+// 4 bits: from the ring.
+__device__ __forceinline__ void load_keys(Keys<4>& x, const Packed& p) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      x.k[r] = __ldcg(reinterpret_cast<const uint4*>(kt + (row0 + g + 8 * r) * 64) + t);
-      x.ks[r] = __ldcg(reinterpret_cast<const uint2*>(ks) + row0 + g + 8 * r);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x.v[i] = __ldcg(reinterpret_cast<const uint4*>(vt + (row0 + v_pos(t, i)) * 64) + (g >> 1));
-      x.vs[i] = __ldcg(reinterpret_cast<const uint2*>(vs) + row0 + v_pos(t, i));
-    }
+  for (int r = 0; r < 2; ++r) {
+    x.k[r] = p.k[(g + 8 * r) * 4 + t];
+    x.ks[r] = p.ks[g + 8 * r];
   }
+}
+__device__ __forceinline__ void load_values(Values<4>& x, const Packed& p) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.v[i] = p.v[v_pos(t, i) * 4 + (g >> 1)];
+    x.vs[i] = p.vs[v_pos(t, i)];
+  }
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
@@ -119,14 +182,17 @@ __device__ __forceinline__ float scale_of(const uint2& s, int j) {
 }
 
 // Query fragments: column g = (head g / 2, part g % 2), dims as a lane of K
-// holds them. [..][1] (fp32 rows): the third part, in the even columns.
-template <bool F32>
+// holds them. [..][2, 3] (fp32 rows): the third part, in the even columns.
+// bias (4 bits, bf16 rows): -24 times the sum over each group of 32 dims of the
+// query of head t: the score of the 16 + code - 24 that the nibbles stand for.
+template <int BITS, bool F32>
 struct Query {
   uint32_t b[8][F32 ? 4 : 2];
+  float bias[BITS == 4 && !F32 ? 4 : 1];
 };
 
 template <int BITS, bool F32>
-__device__ __forceinline__ void load_query(Query<F32>& q, const void* p, long long off, bool in) {
+__device__ __forceinline__ void load_query(Query<BITS, F32>& q, const void* p, long long off, bool in) {
   const int lane = threadIdx.x & 31, t = lane & 3, part = (lane >> 2) & 1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -137,6 +203,12 @@ __device__ __forceinline__ void load_query(Query<F32>& q, const void* p, long lo
                         : make_float4(0.f, 0.f, 0.f, 0.f);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    if constexpr (BITS == 4 && !F32) {
+      float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      q.bias[j] = -24.f * __shfl_sync(0xffffffffu, s, 8 * t);  // from a lane of column 2 t
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       // pairs of the summed index, in the order of the K fragments
@@ -175,7 +247,7 @@ struct Warp {
   float o[8][4];    // O^T: [m-tile][.]
 
   // Scores of positions row g (s0) and g + 8 (s1) for head t.
-  __device__ __forceinline__ void scores(const Tile<BITS>& x, const Query<F32>& q, float& s0,
+  __device__ __forceinline__ void scores(const Keys<BITS>& x, const Query<BITS, F32>& q, float& s0,
                                          float& s1) {
     if constexpr (BITS == 16) {
       float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -188,8 +260,8 @@ struct Warp {
           mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
           if constexpr (F32) mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
         }
-      s0 = c[0] + c[1];
-      s1 = c[2] + c[3];
+      s0 = F32 ? c[0] + c[1] : c[0];
+      s1 = F32 ? c[2] + c[3] : c[2];
     } else {
       s0 = s1 = 0.f;
 #pragma unroll
@@ -198,19 +270,28 @@ struct Warp {
         const uint32_t w0 = word(x.k[0], j), w1 = word(x.k[1], j);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t a[4] = {nibbles(w0, 2 * s), nibbles(w1, 2 * s), nibbles(w0, 2 * s + 1),
-                                 nibbles(w1, 2 * s + 1)};
-          mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
-          if constexpr (F32) mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
+          if constexpr (F32) {
+            const uint32_t a[4] = {nibbles(w0, 2 * s), nibbles(w1, 2 * s), nibbles(w0, 2 * s + 1),
+                                   nibbles(w1, 2 * s + 1)};
+            mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
+            mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
+          } else {
+            const uint32_t a[4] = {nibbles_bf16(w0, 2 * s), nibbles_bf16(w1, 2 * s),
+                                   nibbles_bf16(w0, 2 * s + 1), nibbles_bf16(w1, 2 * s + 1)};
+            if (s == 0)
+              mma16816_from(c, a, q.b[2 * j][0], q.b[2 * j][1], q.bias[j], q.bias[j]);
+            else
+              mma16816(c, a, q.b[2 * j + 1][0], q.b[2 * j + 1][1]);
+          }
         }
-        s0 = fmaf(scale_of(x.ks[0], j), c[0] + c[1], s0);
-        s1 = fmaf(scale_of(x.ks[1], j), c[2] + c[3], s1);
+        s0 = fmaf(scale_of(x.ks[0], j), F32 ? c[0] + c[1] : c[0], s0);
+        s1 = fmaf(scale_of(x.ks[1], j), F32 ? c[2] + c[3] : c[2], s1);
       }
     }
   }
 
   // O^T += V^T P^T; w[i]: this column's weights at v_pos(t, i).
-  __device__ __forceinline__ void values(const Tile<BITS>& x, const float (&w)[4]) {
+  __device__ __forceinline__ void values(const Values<BITS>& x, const float (&w)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, part = g & 1;
     if constexpr (BITS == 16) {
       uint32_t t0 = 0u, t1 = 0u;
@@ -230,6 +311,43 @@ struct Warp {
       }
     } else {
       const unsigned sel = part ? 0x7632u : 0x5410u;  // g odd: the word's upper four dims
+      if constexpr (!F32) {
+        // scales (bf16 bits) of this lane's positions: the largest past 2^12 (or not
+        // a number, or negative), or all of them below 2^-11, where fp16's multiples
+        // of 2^-24 begin to show
+        unsigned top = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, __vmaxu2(x.vs[i].x, x.vs[i].y));
+        top = max(top & 0xffffu, top >> 16);
+        const bool odd = top > 0x4580u || (top != 0u && top < 0x3a00u);
+        if (!__any_sync(0xffffffffu, odd)) {
+          const __half2 p0 = __floats2half2_rn(w[0], w[1]), p1 = __floats2half2_rn(w[2], w[3]);
+          const uint32_t b0 = part ? 0u : *reinterpret_cast<const uint32_t*>(&p0);
+          const uint32_t b1 = part ? 0u : *reinterpret_cast<const uint32_t*>(&p1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // (16 + code) * s - 24 s, one rounding of an exact value
+            const __half2 s0 = __floats2half2_rn(scale_of(x.vs[0], j), scale_of(x.vs[1], j));
+            const __half2 s1 = __floats2half2_rn(scale_of(x.vs[2], j), scale_of(x.vs[3], j));
+            const __half2 m24 = __floats2half2_rn(-24.f, -24.f);
+            const __half2 z0 = __hmul2(s0, m24), z1 = __hmul2(s1, m24);
+            const uint32_t y0 = __byte_perm(word(x.v[0], j), word(x.v[1], j), sel);
+            const uint32_t y1 = __byte_perm(word(x.v[2], j), word(x.v[3], j), sel);
+            auto val = [](uint32_t y, int i, __half2 s, __half2 z) {
+              const uint32_t u = nibbles_half(y, i);
+              const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&u), s, z);
+              return *reinterpret_cast<const uint32_t*>(&v);
+            };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a[4] = {val(y0, 2 * i, s0, z0), val(y0, 2 * i + 1, s0, z0),
+                                     val(y1, 2 * i, s1, z1), val(y1, 2 * i + 1, s1, z1)};
+              mma16816_half(o[2 * j + i], a, b0, b1);
+            }
+          }
+          return;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t t0 = 0u, t1 = 0u;
@@ -263,12 +381,17 @@ struct Partial {
   float o[kStepHeads][kKvDim];
 };
 
+// CTAs on an SM: what the registers of the form allow.
 template <int BITS, bool F32>
-__global__ void __launch_bounds__(kStepThreads, 1)
+constexpr int kStepCtas = BITS == 4 && !F32 ? 4 : 3;
+
+template <int BITS, bool F32>
+__global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
     k_kv_step(KvArgs c, KvRows r, KvAttend a, int chunks) {
-  constexpr int TILES = BITS == 16 ? 1 : 2;  // tiles in flight per step: registers
   __shared__ Partial s_warp[kStepWarps];
   __shared__ Partial s_cta;
+  __shared__ Packed s_ring[BITS == 4 ? kStepWarps : 1][BITS == 4 ? kRing : 1];
+  __shared__ uint64_t s_full[kStepWarps][kRing];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -280,7 +403,7 @@ __global__ void __launch_bounds__(kStepThreads, 1)
   const KvPlace at = kv_place(c, r, row, false);
   // uniform over the cluster: the decision depends on the row alone
   if (at.group < 0 || (a.halt && __ldcg(a.halt + (long long)at.group * a.halt_stride))) return;
-  Query<F32> q;
+  Query<BITS, F32> q;
   load_query<BITS, F32>(q, a.q.p, (long long)row * a.q.row + (long long)(qh0 + (g >> 1)) * a.q.head,
                         (g >> 1) < heads);
   // visible tiles: [0, ns) and [ws, pos / 16]
@@ -297,74 +420,109 @@ __global__ void __launch_bounds__(kStepThreads, 1)
     for (int k = 0; k < 4; ++k) acc.o[i][k] = 0.f;
 
   const int stride = ctas * kStepWarps, wg = rank * kStepWarps + warp;
-  const int steps = total > wg * TILES ? (total - wg * TILES + stride * TILES - 1) / (stride * TILES) : 0;
-  auto tile_of = [&](int it, int u) {
-    const int i = (it * stride + wg) * TILES + u;
+  const int steps = total > wg ? (total - wg + stride - 1) / stride : 0;
+  auto tile_of = [&](int it) {
+    const int i = it * stride + wg;
     return i >= total ? -1 : i < ns ? i : i - ns + ws;
   };
-  const long long tile_bytes = kv_tile_bytes(c.g), page_bytes = kv_page_bytes(c.g);
+  const long long page_bytes = kv_page_bytes(c.g);
   const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
-  const unsigned char* vbase = kbase + tile_bytes * c.g.kv_heads;
-  int pages[TILES];  // lane i: the page of tile tile_of(32 * block + i, u)
-  Tile<BITS> cur[TILES], nxt[TILES];
-  auto fetch = [&](int it, Tile<BITS> (&x)[TILES]) {
-    if ((it & 31) == 0) {
-#pragma unroll
-      for (int u = 0; u < TILES; ++u) {
-        const int tl = tile_of(it + lane, u);
-        pages[u] = tl >= 0 ? kv_page(c, at.seq, (tl * kTile) >> c.g.shift) : -1;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) {
-      // a tile that is not there is read from page 0 and masked
-      const int page = max(0, __shfl_sync(0xffffffffu, pages[u], it & 31));
-      const int tl = max(0, tile_of(it, u));
-      load_tile<BITS>(x[u], kbase + page * page_bytes, vbase + page * page_bytes,
-                      (tl * kTile) & ((1 << c.g.shift) - 1), c.g.shift);
+  const long long v_off = kv_tile_bytes(c.g) * c.g.kv_heads;  // from K's tile to V's
+  const int mask = (1 << c.g.shift) - 1;
+  int pages = -1;  // lane i: the page of step 32 * block + i
+  auto refill = [&](int it) {
+    const int tl = tile_of(it + lane);
+    pages = tl >= 0 ? kv_page(c, at.seq, (tl * kTile) >> c.g.shift) : -1;
+  };
+  // K rows of a step's tile; a tile without a page is read from page 0 and masked.
+  unsigned there = 0u;  // bit it % 32: the tile of step it has a page
+  auto rows_of = [&](int it) {
+    if ((it & 31) == 0) refill(it);
+    const int page = __shfl_sync(0xffffffffu, pages, it & 31);
+    there = (there & ~(1u << (it & 31))) | (unsigned)(page >= 0) << (it & 31);
+    const int row = (max(0, tile_of(it)) * kTile) & mask;
+    return kbase + max(0, page) * page_bytes + row * (BITS == 16 ? 2 * kKvDim : kKvCodeBytes);
+  };
+  Keys<BITS> kx;
+  Values<BITS> vx;
+  const unsigned char* cur = kbase;
+  // 4 bits: starts the copies of step it's tile
+  auto start = [&](int it) {
+    const unsigned char* k = rows_of(it);
+    if (lane == 0) {
+      Packed& p = s_ring[BITS == 4 ? warp : 0][BITS == 4 ? it % kRing : 0];
+      uint64_t* bar = &s_full[warp][it % kRing];
+      const int row = (max(0, tile_of(it)) * kTile) & mask;
+      // from a row's codes to its scales
+      const int to_scales = (kKvCodeBytes << c.g.shift) - row * (kKvCodeBytes - 2 * kKvGroups);
+      mbar_expect_tx(bar, sizeof(Packed));
+      bulk_g2s(p.k, k, sizeof p.k, bar);
+      bulk_g2s(p.ks, k + to_scales, sizeof p.ks, bar);
+      bulk_g2s(p.v, k + v_off, sizeof p.v, bar);
+      bulk_g2s(p.vs, k + v_off + to_scales, sizeof p.vs, bar);
     }
   };
-  auto have = [&](int it, int u) {  // before the pages of the next block are fetched
-    return __shfl_sync(0xffffffffu, pages[u], it & 31) >= 0;
-  };
-  if (steps) fetch(0, cur);
+  if constexpr (BITS == 4) {
+    if (lane == 0)
+      for (int i = 0; i < kRing; ++i) mbar_init(&s_full[warp][i], 1);
+    fence_mbar_init();
+    __syncwarp();
+    for (int i = 0; i < kRing && i < steps; ++i) start(i);
+  } else if (steps) {
+    cur = rows_of(0);
+    load_keys(kx, cur);
+    load_values(vx, cur + v_off);
+  }
   for (int it = 0; it < steps; ++it) {
-    bool there[TILES];
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) there[u] = have(it, u);
-    if (it + 1 < steps) fetch(it + 1, nxt);
-    float s[TILES][2];
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) {
-      acc.scores(cur[u], q, s[u][0], s[u][1]);
-      s[u][0] *= a.scale;
-      s[u][1] *= a.scale;
-      const int p0 = tile_of(it, u) * kTile;
-      const bool full = there[u] && p0 + kTile - 1 <= at.pos &&
-                        (a.window == 0 || p0 > at.pos - a.window || p0 + kTile <= a.sinks);
-      if (!full) {
-        auto vis = [&](int p) { return there[u] && kv_sees(at.pos, p, a.window, a.sinks); };
-        if (!vis(p0 + g)) s[u][0] = -INFINITY;
-        if (!vis(p0 + g + 8)) s[u][1] = -INFINITY;
-        // what a masked row holds must not meet its zero weight: it may be NaN
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!vis(p0 + v_pos(t, i))) {
-            if constexpr (BITS == 16)
-              cur[u].v[i][0] = cur[u].v[i][1] = make_uint4(0u, 0u, 0u, 0u);
-            else
-              cur[u].vs[i] = make_uint2(0u, 0u);
-          }
+    float s[2];
+    const bool is_there = (there >> (it & 31)) & 1u;
+    if constexpr (BITS == 4) {
+      const Packed& p = s_ring[warp][it % kRing];
+      const bool landed = mbar_wait_cycles(&s_full[warp][it % kRing], (it / kRing) & 1, kStepWaitCycles);
+      if (!__all_sync(0xffffffffu, landed)) {
+        kv_status(c, kKvTimeout);
+        for (int i = it + 1; i < min(it + kRing, steps); ++i)  // no copy may outlive the CTA
+          mbar_wait_cycles(&s_full[warp][i % kRing], (i / kRing) & 1, kStepWaitCycles);
+        break;
       }
-      top = fmaxf(top, fmaxf(s[u][0], s[u][1]));
+      load_keys(kx, p);
+      load_values(vx, p);
+      __syncwarp();  // every lane has its values: the slot may be filled again
+      if (it + kRing < steps) start(it + kRing);
+      acc.scores(kx, q, s[0], s[1]);
+    } else {
+      acc.scores(kx, q, s[0], s[1]);
+      if (it + 1 < steps) {
+        cur = rows_of(it + 1);
+        load_keys(kx, cur);
+      }
     }
+    s[0] *= a.scale;
+    s[1] *= a.scale;
+    const int p0 = tile_of(it) * kTile;
+    const bool full = is_there && p0 + kTile - 1 <= at.pos &&
+                      (a.window == 0 || p0 > at.pos - a.window || p0 + kTile <= a.sinks);
+    if (!full) {
+      auto vis = [&](int p) { return is_there && kv_sees(at.pos, p, a.window, a.sinks); };
+      if (!vis(p0 + g)) s[0] = -INFINITY;
+      if (!vis(p0 + g + 8)) s[1] = -INFINITY;
+      // what a masked row holds must not meet its zero weight: it may be NaN
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!vis(p0 + v_pos(t, i))) {
+          if constexpr (BITS == 16)
+            vx.v[i][0] = vx.v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+          else
+            vx.vs[i] = make_uint2(0u, 0u);
+        }
+    }
+    float top = fmaxf(s[0], s[1]);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (__any_sync(0xffffffffu, top > acc.m)) {
       const float m = fmaxf(acc.m, top);
       // no finite score yet: nothing to rescale (and -inf - -inf is not a number)
-      const float f = m == -INFINITY ? 1.f : exp2f((acc.m - m) * 1.4426950408889634f);
+      const float f = m == -INFINITY ? 1.f : exp2_fast((acc.m - m) * 1.4426950408889634f);
       acc.m = m;
       acc.l *= f;
 #pragma unroll
@@ -373,23 +531,21 @@ __global__ void __launch_bounds__(kStepThreads, 1)
         for (int k = 0; k < 4; ++k) acc.o[i][k] *= f;
     }
     const float ref = acc.m == -INFINITY ? 0.f : acc.m;
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) {
-      const float w0 = exp2f((s[u][0] - ref) * 1.4426950408889634f);
-      const float w1 = exp2f((s[u][1] - ref) * 1.4426950408889634f);
-      acc.l += w0 + w1;
-      // weights of (positions 2 t, 2 t + 1 and + 8; head g / 2): from the lanes
-      // that hold them as (position g', head t')
-      float w[4];
-      const int src = 8 * t + (g >> 1);
-      w[0] = __shfl_sync(0xffffffffu, w0, src);
-      w[1] = __shfl_sync(0xffffffffu, w0, src + 4);
-      w[2] = __shfl_sync(0xffffffffu, w1, src);
-      w[3] = __shfl_sync(0xffffffffu, w1, src + 4);
-      acc.values(cur[u], w);
+    const float w0 = exp2_fast((s[0] - ref) * 1.4426950408889634f);
+    const float w1 = exp2_fast((s[1] - ref) * 1.4426950408889634f);
+    acc.l += w0 + w1;
+    // weights of (positions v_pos(t, i); head g / 2): from the lanes that hold
+    // them as (position g' or g' + 8, head t')
+    float w[4];
+    const int src = 4 * t + (g >> 1);
+    w[0] = __shfl_sync(0xffffffffu, w0, src);
+    w[1] = __shfl_sync(0xffffffffu, w0, src + 16);
+    w[2] = __shfl_sync(0xffffffffu, w1, src);
+    w[3] = __shfl_sync(0xffffffffu, w1, src + 16);
+    acc.values(vx, w);
+    if constexpr (BITS == 16) {
+      if (it + 1 < steps) load_values(vx, cur + v_off);
     }
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) cur[u] = nxt[u];
   }
 
   // warp -> CTA
@@ -425,7 +581,7 @@ __global__ void __launch_bounds__(kStepThreads, 1)
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w) {
-      const float f = exp2f((s_warp[w].m[h] - ref) * 1.4426950408889634f);
+      const float f = exp2_fast((s_warp[w].m[h] - ref) * 1.4426950408889634f);
       l = fmaf(f, s_warp[w].l[h], l);
       o = fmaf(f, s_warp[w].o[h][d], o);
     }
@@ -448,7 +604,7 @@ __global__ void __launch_bounds__(kStepThreads, 1)
     for (int k = 0; k < ctas; ++k) m = fmaxf(m, ld_cluster_f32(cluster_map(&s_cta.m[h], k)));
     const float ref = m == -INFINITY ? 0.f : m;
     for (int k = 0; k < ctas; ++k) {
-      const float f = exp2f((ld_cluster_f32(cluster_map(&s_cta.m[h], k)) - ref) * 1.4426950408889634f);
+      const float f = exp2_fast((ld_cluster_f32(cluster_map(&s_cta.m[h], k)) - ref) * 1.4426950408889634f);
       l = fmaf(f, ld_cluster_f32(cluster_map(&s_cta.l[h], k)), l);
       o = fmaf(f, ld_cluster_f32(cluster_map(&s_cta.o[h][d], k)), o);
     }
@@ -461,7 +617,6 @@ __global__ void __launch_bounds__(kStepThreads, 1)
 
 template <int BITS, bool F32>
 cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream_t stream) {
-  constexpr int TILES = BITS == 16 ? 1 : 2;
   auto kernel = k_kv_step<BITS, F32>;
   // clusters of 16 are past the portable size: asked for once per device
   static std::mutex mu;
@@ -480,15 +635,27 @@ cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream
   }
   const int group = a.q_heads / c.g.kv_heads;
   const int chunks = (group + kStepHeads - 1) / kStepHeads;
-  // Split a row's positions over a cluster until every SM has a CTA, as long
-  // as every warp still has a step of its own.
+  // How many CTAs share a row's positions: the least time by a model of waves,
+  // each a fixed part (3 us: tables, first loads, merging) and a part per tile
+  // of a warp (0.5 us with every warp of the SM at work). More CTAs shorten a
+  // wave and may add one; fewer than a tile per warp is never worth it.
   const long long units = (long long)r.rows * c.g.kv_heads * chunks;
   long long longest = kv_capacity(c.g);
   if (r.max_length) longest = std::min<long long>(longest, r.max_length);
   if (a.window) longest = std::min<long long>(longest, (long long)a.window + a.sinks + 2 * kTile);
-  const long long per_cta = (long long)kStepWarps * TILES * kTile;
+  const long long tiles = (longest + kTile - 1) / kTile, slots = 148LL * kStepCtas<BITS, F32>;
   int ctas = 1;
-  while (ctas < kMaxCluster && units * ctas < 148 && longest > per_cta * ctas) ctas *= 2;
+  double best = 1e300;
+  for (int n = 1; n <= kMaxCluster; n *= 2) {
+    if (n > 1 && tiles <= (long long)kStepWarps * (n / 2)) break;
+    const double waves = (double)((units * n + slots - 1) / slots);
+    const double per_warp = (double)((tiles + (long long)n * kStepWarps - 1) / (n * kStepWarps));
+    const double us = waves * (3.0 + 0.5 * per_warp);
+    if (us < best) {
+      best = us;
+      ctas = n;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(r.rows * (long long)ctas), (unsigned)(c.g.kv_heads * chunks));
   cfg.blockDim = dim3(kStepThreads);

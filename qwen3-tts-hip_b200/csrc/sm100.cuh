@@ -76,6 +76,13 @@ __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, unsigned by
       "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
       : "memory");
 }
+__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
 // 2-D tiled tensor copy global -> this CTA's shared memory; x is the innermost
 // coordinate in elements (callers keep x * element size a multiple of 16 B).
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, int y,
