@@ -16,17 +16,20 @@
 // Column pairs 2 t, 2 t + 1 of an accumulator sit in one lane: summing the
 // parts costs one addition.
 //
-// 4-bit rows: codes become small integers by bit operations, a code's nibble
-// placed in the mantissa of 16. K: each group of 32 dims accumulates apart and
-// its scale multiplies the fp32 sum. V, fp32 rows: the scale multiplies the fp32
-// weight before it is split into parts. V, bf16 rows: code * scale is exact in
-// fp16 (11 bits) for scales of 2^-14 to 2^12, and weights are rounded to fp16
-// (2^-12); a tile with other scales takes the first way.
+// 4-bit rows: codes become small integers by bit operations, which run at half
+// rate and bound the 4-bit form (an and-or per pair of codes, a shift for half
+// of them). K: each group of 32 dims accumulates apart and its scale multiplies
+// the fp32 sum. V: the scale multiplies the fp32 weight.
+//   bf16 rows: fp16 operands, a nibble in place in the mantissa of 64.0. K: 64 +
+//   code is used as it is and 72 times the query's sum is taken off the fp32
+//   accumulator; V: 72 is taken off (exact). Weight times scale is rounded to
+//   fp16 (2^-12): scales past 2^12, or all below 2^-11, take the form below.
+//   fp32 rows: code - 8 in bf16 (exact), weight times scale in three parts.
 //
-// Bound by bytes in flight and by issue. 4-bit tiles (four contiguous pieces,
-// 2,304 bytes) come by bulk copies into a ring of each warp's own, kRing tiles
-// ahead; 16-bit ones into registers, refilled in place: the next K while its
-// weights meet V, the next V while its K is scored.
+// 16-bit tiles come into registers, refilled in place: the next K while its
+// weights meet V, the next V while its K is scored. 4-bit rows come 32 at a time
+// (four contiguous pieces, 4,608 bytes) by bulk copies into a ring of each
+// warp's own.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
 // CTAs of a cluster through distributed shared memory, both in a fixed order.
@@ -46,7 +49,7 @@ namespace {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = kStepWarps * 32;
 constexpr int kStepHeads = 4;   // query heads of one CTA
-constexpr int kRing = 4;        // 4-bit tiles in flight per warp
+constexpr int kRing = 2;        // 4-bit units of 32 positions in flight per warp
 constexpr int kTile = 16;       // positions of one matrix instruction; a page is a multiple
 constexpr int kMaxCluster = 16;
 constexpr long long kStepWaitCycles = 4000000000ll;  // two seconds at 2 GHz
@@ -63,10 +66,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+__device__ __forceinline__ void mma16816_half_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                               uint32_t b1, float c0, float c2) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
       " {%10,%11,%12,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(0.f), "f"(c2));
@@ -82,17 +85,18 @@ __device__ __forceinline__ void mma16816_half(float (&c)[4], const uint32_t (&a)
 __device__ __forceinline__ uint32_t shifted(uint32_t w, int left) {
   return left >= 0 ? w << left : w >> -left;
 }
-// Nibble i of each 16-bit half of w as 16 + code: the nibble in the upper
-// mantissa bits of 16.0, bf16 (bits 3-6) or fp16 (bits 6-9).
-__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, int i) {
-  return (shifted(w, 3 - 4 * i) & 0x00780078u) | 0x41804180u;
+// Nibble i of each 16-bit half of w as the fp16 64 + code (mantissa bits 4-7).
+__device__ __forceinline__ uint32_t nibbles_64(uint32_t w, int i) {
+  return (shifted(w, 4 - 4 * i) & 0x00f000f0u) | 0x54005400u;
 }
+// As code - 8, exact, in fp16 or bf16 (there from 16 + code, mantissa bits 3-6).
 __device__ __forceinline__ uint32_t nibbles_half(uint32_t w, int i) {
-  return (shifted(w, 6 - 4 * i) & 0x03c003c0u) | 0x4c004c00u;
+  const uint32_t u = nibbles_64(w, i);
+  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(-72.f, -72.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
-// The same as n = code - 8, exact.
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
-  const uint32_t u = nibbles_bf16(w, i);
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, int i) {
+  const uint32_t u = (shifted(w, 3 - 4 * i) & 0x00780078u) | 0x41804180u;
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
                                    __nv_bfloat162(__float2bfloat16(24.f), __float2bfloat16(24.f)));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -127,10 +131,11 @@ struct Values<4> {
 // of a 4-bit tile at two to a bank.
 __device__ __forceinline__ int v_pos(int t, int i) { return t + 4 * i; }
 
-// A 4-bit tile in shared memory.
+// A 4-bit unit in shared memory.
+constexpr int kUnit = 2 * kTile;
 struct __align__(16) Packed {
-  uint4 k[kTile * 4], v[kTile * 4];  // 64 bytes a row
-  uint2 ks[kTile], vs[kTile];
+  uint4 k[kUnit * 4], v[kUnit * 4];  // 64 bytes a row
+  uint2 ks[kUnit], vs[kUnit];
 };
 
 // 16 bits: rows of a K (V) tile from global memory.
@@ -151,20 +156,20 @@ __device__ __forceinline__ void load_values(Values<16>& x, const unsigned char* 
       x.v[i][h] = __ldcg(reinterpret_cast<const uint4*>(rows + v_pos(t, i) * 256) + 8 * h + g);
 }
 // 4 bits: from the ring.
-__device__ __forceinline__ void load_keys(Keys<4>& x, const Packed& p) {
+__device__ __forceinline__ void load_keys(Keys<4>& x, const Packed& p, int row0) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    x.k[r] = p.k[(g + 8 * r) * 4 + t];
-    x.ks[r] = p.ks[g + 8 * r];
+    x.k[r] = p.k[(row0 + g + 8 * r) * 4 + t];
+    x.ks[r] = p.ks[row0 + g + 8 * r];
   }
 }
-__device__ __forceinline__ void load_values(Values<4>& x, const Packed& p) {
+__device__ __forceinline__ void load_values(Values<4>& x, const Packed& p, int row0) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x.v[i] = p.v[v_pos(t, i) * 4 + (g >> 1)];
-    x.vs[i] = p.vs[v_pos(t, i)];
+    x.v[i] = p.v[(row0 + v_pos(t, i)) * 4 + (g >> 1)];
+    x.vs[i] = p.vs[row0 + v_pos(t, i)];
   }
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -183,17 +188,39 @@ __device__ __forceinline__ float scale_of(const uint2& s, int j) {
 
 // Query fragments: column g = (head g / 2, part g % 2), dims as a lane of K
 // holds them. [..][2, 3] (fp32 rows): the third part, in the even columns.
-// bias (4 bits, bf16 rows): -24 times the sum over each group of 32 dims of the
-// query of head t: the score of the 16 + code - 24 that the nibbles stand for.
+// 4 bits, bf16 rows: in fp16, the row scaled by a power of two (exact: 8 bits);
+// bias: -72 times the sum over each group of 32 dims of the query of head t;
+// unscale: of head t.
 template <int BITS, bool F32>
 struct Query {
+  static constexpr bool kHalf = BITS == 4 && !F32;
   uint32_t b[8][F32 ? 4 : 2];
-  float bias[BITS == 4 && !F32 ? 4 : 1];
+  float bias[kHalf ? 4 : 1];
+  float unscale = 1.f;
 };
 
 template <int BITS, bool F32>
 __device__ __forceinline__ void load_query(Query<BITS, F32>& q, const void* p, long long off, bool in) {
   const int lane = threadIdx.x & 31, t = lane & 3, part = (lane >> 2) & 1;
+  float up = 1.f;
+  if constexpr (Query<BITS, F32>::kHalf) {
+    float top = 0.f;
+#pragma unroll
+    for (int d = 0; d < 32; d += 4) {
+      const float4 a = in ? kv_load4(p, off + 32 * t + d, KV_BF16) : make_float4(0.f, 0.f, 0.f, 0.f);
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float down = 1.f;
+    if (top > 0.f && isfinite(top)) {
+      // largest magnitude into [2^8, 2^9); the limits keep both factors normal
+      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -110), 110);
+      up = __uint_as_float((unsigned)(127 + 8 - e) << 23);
+      down = __uint_as_float((unsigned)(127 - 8 + e) << 23);
+    }
+    q.unscale = __shfl_sync(0xffffffffu, down, 8 * t);  // from a lane of column 2 t
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float x[8];
@@ -203,11 +230,16 @@ __device__ __forceinline__ void load_query(Query<BITS, F32>& q, const void* p, l
                         : make_float4(0.f, 0.f, 0.f, 0.f);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    if constexpr (BITS == 4 && !F32) {
-      float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    if constexpr (Query<BITS, F32>::kHalf) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= up;
+        s += x[i];
+      }
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
-      q.bias[j] = -24.f * __shfl_sync(0xffffffffu, s, 8 * t);  // from a lane of column 2 t
+      q.bias[j] = -72.f * __shfl_sync(0xffffffffu, s, 8 * t);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -218,7 +250,10 @@ __device__ __forceinline__ void load_query(Query<BITS, F32>& q, const void* p, l
       for (int w = 0; w < 2; ++w) {
         const int* d = BITS == 16 ? pair16[2 * s + w] : pair4[2 * s + w];
         const float lo = x[d[0]], hi = x[d[1]];
-        if constexpr (!F32) {
+        if constexpr (Query<BITS, F32>::kHalf) {
+          const __half2 v = __floats2half2_rn(lo, hi);
+          q.b[2 * j + s][w] = part ? 0u : *reinterpret_cast<const uint32_t*>(&v);
+        } else if constexpr (!F32) {
           q.b[2 * j + s][w] = part ? 0u : pack_bf16(lo, hi);
         } else {
           const float l1 = bf16_round(lo), h1 = bf16_round(hi);
@@ -271,17 +306,17 @@ struct Warp {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if constexpr (F32) {
-            const uint32_t a[4] = {nibbles(w0, 2 * s), nibbles(w1, 2 * s), nibbles(w0, 2 * s + 1),
-                                   nibbles(w1, 2 * s + 1)};
+            const uint32_t a[4] = {nibbles_bf16(w0, 2 * s), nibbles_bf16(w1, 2 * s),
+                                   nibbles_bf16(w0, 2 * s + 1), nibbles_bf16(w1, 2 * s + 1)};
             mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
             mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
           } else {
-            const uint32_t a[4] = {nibbles_bf16(w0, 2 * s), nibbles_bf16(w1, 2 * s),
-                                   nibbles_bf16(w0, 2 * s + 1), nibbles_bf16(w1, 2 * s + 1)};
+            const uint32_t a[4] = {nibbles_64(w0, 2 * s), nibbles_64(w1, 2 * s),
+                                   nibbles_64(w0, 2 * s + 1), nibbles_64(w1, 2 * s + 1)};
             if (s == 0)
-              mma16816_from(c, a, q.b[2 * j][0], q.b[2 * j][1], q.bias[j], q.bias[j]);
+              mma16816_half_from(c, a, q.b[2 * j][0], q.b[2 * j][1], q.bias[j], q.bias[j]);
             else
-              mma16816(c, a, q.b[2 * j + 1][0], q.b[2 * j + 1][1]);
+              mma16816_half(c, a, q.b[2 * j + 1][0], q.b[2 * j + 1][1]);
           }
         }
         s0 = fmaf(scale_of(x.ks[0], j), F32 ? c[0] + c[1] : c[0], s0);
@@ -291,7 +326,8 @@ struct Warp {
   }
 
   // O^T += V^T P^T; w[i]: this column's weights at v_pos(t, i).
-  __device__ __forceinline__ void values(const Values<BITS>& x, const float (&w)[4]) {
+  // plain (4 bits, bf16 rows): every scale of the unit suits fp16.
+  __device__ __forceinline__ void values(const Values<BITS>& x, const float (&w)[4], bool plain) {
     const int lane = threadIdx.x & 31, g = lane >> 2, part = g & 1;
     if constexpr (BITS == 16) {
       uint32_t t0 = 0u, t1 = 0u;
@@ -311,42 +347,23 @@ struct Warp {
       }
     } else {
       const unsigned sel = part ? 0x7632u : 0x5410u;  // g odd: the word's upper four dims
-      if constexpr (!F32) {
-        // scales (bf16 bits) of this lane's positions: the largest past 2^12 (or not
-        // a number, or negative), or all of them below 2^-11, where fp16's multiples
-        // of 2^-24 begin to show
-        unsigned top = 0u;
+      if (!F32 && plain) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, __vmaxu2(x.vs[i].x, x.vs[i].y));
-        top = max(top & 0xffffu, top >> 16);
-        const bool odd = top > 0x4580u || (top != 0u && top < 0x3a00u);
-        if (!__any_sync(0xffffffffu, odd)) {
-          const __half2 p0 = __floats2half2_rn(w[0], w[1]), p1 = __floats2half2_rn(w[2], w[3]);
-          const uint32_t b0 = part ? 0u : *reinterpret_cast<const uint32_t*>(&p0);
-          const uint32_t b1 = part ? 0u : *reinterpret_cast<const uint32_t*>(&p1);
+        for (int j = 0; j < 4; ++j) {
+          const __half2 p0 = __floats2half2_rn(w[0] * scale_of(x.vs[0], j), w[1] * scale_of(x.vs[1], j));
+          const __half2 p1 = __floats2half2_rn(w[2] * scale_of(x.vs[2], j), w[3] * scale_of(x.vs[3], j));
+          const uint32_t b0 = *reinterpret_cast<const uint32_t*>(&p0);
+          const uint32_t b1 = *reinterpret_cast<const uint32_t*>(&p1);
+          const uint32_t y0 = __byte_perm(word(x.v[0], j), word(x.v[1], j), sel);
+          const uint32_t y1 = __byte_perm(word(x.v[2], j), word(x.v[3], j), sel);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // (16 + code) * s - 24 s, one rounding of an exact value
-            const __half2 s0 = __floats2half2_rn(scale_of(x.vs[0], j), scale_of(x.vs[1], j));
-            const __half2 s1 = __floats2half2_rn(scale_of(x.vs[2], j), scale_of(x.vs[3], j));
-            const __half2 m24 = __floats2half2_rn(-24.f, -24.f);
-            const __half2 z0 = __hmul2(s0, m24), z1 = __hmul2(s1, m24);
-            const uint32_t y0 = __byte_perm(word(x.v[0], j), word(x.v[1], j), sel);
-            const uint32_t y1 = __byte_perm(word(x.v[2], j), word(x.v[3], j), sel);
-            auto val = [](uint32_t y, int i, __half2 s, __half2 z) {
-              const uint32_t u = nibbles_half(y, i);
-              const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&u), s, z);
-              return *reinterpret_cast<const uint32_t*>(&v);
-            };
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t a[4] = {val(y0, 2 * i, s0, z0), val(y0, 2 * i + 1, s0, z0),
-                                     val(y1, 2 * i, s1, z1), val(y1, 2 * i + 1, s1, z1)};
-              mma16816_half(o[2 * j + i], a, b0, b1);
-            }
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a[4] = {nibbles_half(y0, 2 * i), nibbles_half(y0, 2 * i + 1),
+                                   nibbles_half(y1, 2 * i), nibbles_half(y1, 2 * i + 1)};
+            mma16816_half(o[2 * j + i], a, b0, b1);
           }
-          return;
         }
+        return;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -359,8 +376,8 @@ struct Warp {
         const uint32_t y1 = __byte_perm(word(x.v[2], j), word(x.v[3], j), sel);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t a[4] = {nibbles(y0, 2 * i), nibbles(y0, 2 * i + 1), nibbles(y1, 2 * i),
-                                 nibbles(y1, 2 * i + 1)};
+          const uint32_t a[4] = {nibbles_bf16(y0, 2 * i), nibbles_bf16(y0, 2 * i + 1),
+                                 nibbles_bf16(y1, 2 * i), nibbles_bf16(y1, 2 * i + 1)};
           mma16816(o[2 * j + i], a, b0, b1);
           if constexpr (F32) mma16816(o[2 * j + i], a, t0, t1);
         }
@@ -390,7 +407,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
     k_kv_step(KvArgs c, KvRows r, KvAttend a, int chunks) {
   __shared__ Partial s_warp[kStepWarps];
   __shared__ Partial s_cta;
-  __shared__ Packed s_ring[BITS == 4 ? kStepWarps : 1][BITS == 4 ? kRing : 1];
+  extern __shared__ Packed s_rings[];  // 4 bits: kRing per warp
   __shared__ uint64_t s_full[kStepWarps][kRing];
   pdl_wait();
   pdl_trigger();
@@ -406,11 +423,12 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
   Query<BITS, F32> q;
   load_query<BITS, F32>(q, a.q.p, (long long)row * a.q.row + (long long)(qh0 + (g >> 1)) * a.q.head,
                         (g >> 1) < heads);
-  // visible tiles: [0, ns) and [ws, pos / 16]
+  // visible units (of 16 positions, 32 for 4 bits): [0, ns) and [ws, pos / unit]
+  constexpr int TILES = BITS == 4 ? 2 : 1, UNIT = TILES * kTile;
   const KvSpan sp = kv_span(at.ok ? at.pos : 0, a.window, a.sinks);
-  const int ns = (sp.sink_end + kTile - 1) / kTile;
-  const int ws = max(sp.first / kTile, ns);
-  const int total = at.ok ? ns + at.pos / kTile - ws + 1 : 0;
+  const int ns = (sp.sink_end + UNIT - 1) / UNIT;
+  const int ws = max(sp.first / UNIT, ns);
+  const int total = at.ok ? ns + at.pos / UNIT - ws + 1 : 0;
   Warp<BITS, F32> acc;
   acc.m = -INFINITY;
   acc.l = 0.f;
@@ -421,45 +439,58 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
 
   const int stride = ctas * kStepWarps, wg = rank * kStepWarps + warp;
   const int steps = total > wg ? (total - wg + stride - 1) / stride : 0;
-  auto tile_of = [&](int it) {
+  auto unit_of = [&](int it) {
     const int i = it * stride + wg;
-    return i >= total ? -1 : i < ns ? i : i - ns + ws;
+    return i < ns ? i : i - ns + ws;
   };
   const long long page_bytes = kv_page_bytes(c.g);
   const unsigned char* kbase = c.pool + kv_tile_at(c.g, 0, a.layer, 0, head);
   const long long v_off = kv_tile_bytes(c.g) * c.g.kv_heads;  // from K's tile to V's
   const int mask = (1 << c.g.shift) - 1;
-  int pages = -1;  // lane i: the page of step 32 * block + i
+  // The pages of 32 / TILES units, a tile per lane (-1: none; such a tile is read
+  // from page 0 and masked).
+  constexpr int HELD = 32 / TILES;
+  int pages = -1;
   auto refill = [&](int it) {
-    const int tl = tile_of(it + lane);
-    pages = tl >= 0 ? kv_page(c, at.seq, (tl * kTile) >> c.g.shift) : -1;
-  };
-  // K rows of a step's tile; a tile without a page is read from page 0 and masked.
-  unsigned there = 0u;  // bit it % 32: the tile of step it has a page
-  auto rows_of = [&](int it) {
-    if ((it & 31) == 0) refill(it);
-    const int page = __shfl_sync(0xffffffffu, pages, it & 31);
-    there = (there & ~(1u << (it & 31))) | (unsigned)(page >= 0) << (it & 31);
-    const int row = (max(0, tile_of(it)) * kTile) & mask;
-    return kbase + max(0, page) * page_bytes + row * (BITS == 16 ? 2 * kKvDim : kKvCodeBytes);
+    const int un = it + lane / TILES < steps ? unit_of(it + lane / TILES) : -1;
+    const int p = un * UNIT + lane % TILES * kTile;
+    pages = un >= 0 && p <= at.pos ? kv_page(c, at.seq, p >> c.g.shift) : -1;
   };
   Keys<BITS> kx;
   Values<BITS> vx;
   const unsigned char* cur = kbase;
-  // 4 bits: starts the copies of step it's tile
+  unsigned has = 0u;  // which tiles of a step have a page: TILES bits per ring slot
+  constexpr unsigned ALL = (1u << TILES) - 1u;
+  auto rows_of = [&](int it) {  // 16 bits
+    if (it % HELD == 0) refill(it);
+    const int page = __shfl_sync(0xffffffffu, pages, it % HELD);
+    has = page >= 0;
+    return kbase + max(page, 0) * page_bytes + ((unit_of(it) * UNIT) & mask) * (2 * kKvDim);
+  };
+  // 4 bits: starts the copies of step it's unit, in one piece if a page holds it
+  static_assert((kRing & (kRing - 1)) == 0, "slots by masking");
+  Packed* ring = s_rings + warp * kRing;
+  const int piece = min(mask + 1, kUnit), scales = kKvCodeBytes << c.g.shift;
   auto start = [&](int it) {
-    const unsigned char* k = rows_of(it);
+    if (it % HELD == 0) refill(it);
+    const int slot = it & (kRing - 1), bit = it % HELD * TILES;
+    const int pg0 = __shfl_sync(0xffffffffu, pages, bit);
+    const int pg1 = __shfl_sync(0xffffffffu, pages, bit + TILES - 1);
+    has = (has & ~(ALL << (slot * TILES))) | ((pg0 >= 0) | (pg1 >= 0) << 1) << (slot * TILES);
     if (lane == 0) {
-      Packed& p = s_ring[BITS == 4 ? warp : 0][BITS == 4 ? it % kRing : 0];
-      uint64_t* bar = &s_full[warp][it % kRing];
-      const int row = (max(0, tile_of(it)) * kTile) & mask;
-      // from a row's codes to its scales
-      const int to_scales = (kKvCodeBytes << c.g.shift) - row * (kKvCodeBytes - 2 * kKvGroups);
+      Packed& p = ring[slot];
+      uint64_t* bar = &s_full[warp][slot];
       mbar_expect_tx(bar, sizeof(Packed));
-      bulk_g2s(p.k, k, sizeof p.k, bar);
-      bulk_g2s(p.ks, k + to_scales, sizeof p.ks, bar);
-      bulk_g2s(p.v, k + v_off, sizeof p.v, bar);
-      bulk_g2s(p.vs, k + v_off + to_scales, sizeof p.vs, bar);
+      const int row = (unit_of(it) * UNIT) & mask;
+      for (int u = 0; u < kUnit; u += piece) {  // pieces of 16 start a page
+        const unsigned char* tile = kbase + max(u ? pg1 : pg0, 0) * page_bytes;
+        const unsigned char* k = tile + row * kKvCodeBytes;
+        const unsigned char* ks = tile + scales + row * 2 * kKvGroups;
+        bulk_g2s(p.k + 4 * u, k, piece * kKvCodeBytes, bar);
+        bulk_g2s(p.ks + u, ks, piece * 2 * kKvGroups, bar);
+        bulk_g2s(p.v + 4 * u, k + v_off, piece * kKvCodeBytes, bar);
+        bulk_g2s(p.vs + u, ks + v_off, piece * 2 * kKvGroups, bar);
+      }
     }
   };
   if constexpr (BITS == 4) {
@@ -474,49 +505,56 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
     load_values(vx, cur + v_off);
   }
   for (int it = 0; it < steps; ++it) {
-    float s[2];
-    const bool is_there = (there >> (it & 31)) & 1u;
+    float s[TILES][2];
+    const int slot = it & (kRing - 1);
+    const unsigned mine = BITS == 4 ? has >> (slot * TILES) & ALL : has;
+    const Packed& p = ring[slot];
+    bool plain = true;
     if constexpr (BITS == 4) {
-      const Packed& p = s_ring[warp][it % kRing];
-      const bool landed = mbar_wait_cycles(&s_full[warp][it % kRing], (it / kRing) & 1, kStepWaitCycles);
+      const bool landed = mbar_wait_cycles(&s_full[warp][slot], (it / kRing) & 1, kStepWaitCycles);
       if (!__all_sync(0xffffffffu, landed)) {
         kv_status(c, kKvTimeout);
         for (int i = it + 1; i < min(it + kRing, steps); ++i)  // no copy may outlive the CTA
           mbar_wait_cycles(&s_full[warp][i % kRing], (i / kRing) & 1, kStepWaitCycles);
         break;
       }
-      load_keys(kx, p);
-      load_values(vx, p);
-      __syncwarp();  // every lane has its values: the slot may be filled again
-      if (it + kRing < steps) start(it + kRing);
-      acc.scores(kx, q, s[0], s[1]);
+      if constexpr (!F32) {
+        // the four scales of V's row `lane` (bf16 bits): past 2^12, not a number or
+        // negative; or all below 2^-11, where fp16's multiples of 2^-24 begin to show
+        const uint2 vs = p.vs[lane];
+        const unsigned top = max(max(vs.x & 0xffffu, vs.x >> 16), max(vs.y & 0xffffu, vs.y >> 16));
+        plain = !__any_sync(0xffffffffu, top > 0x4580u || (top != 0u && top < 0x3a00u));
+      }
+#pragma unroll
+      for (int u = 0; u < TILES; ++u) {
+        load_keys(kx, p, u * kTile);
+        acc.scores(kx, q, s[u][0], s[u][1]);
+      }
     } else {
-      acc.scores(kx, q, s[0], s[1]);
+      acc.scores(kx, q, s[0][0], s[0][1]);
       if (it + 1 < steps) {
         cur = rows_of(it + 1);
         load_keys(kx, cur);
       }
     }
-    s[0] *= a.scale;
-    s[1] *= a.scale;
-    const int p0 = tile_of(it) * kTile;
-    const bool full = is_there && p0 + kTile - 1 <= at.pos &&
-                      (a.window == 0 || p0 > at.pos - a.window || p0 + kTile <= a.sinks);
-    if (!full) {
-      auto vis = [&](int p) { return is_there && kv_sees(at.pos, p, a.window, a.sinks); };
-      if (!vis(p0 + g)) s[0] = -INFINITY;
-      if (!vis(p0 + g + 8)) s[1] = -INFINITY;
-      // what a masked row holds must not meet its zero weight: it may be NaN
+    const float by = a.scale * q.unscale;
+    const int p0 = unit_of(it) * UNIT;
+    const bool full = mine == ALL && p0 + UNIT - 1 <= at.pos &&
+                      (a.window == 0 || p0 > at.pos - a.window || p0 + UNIT <= a.sinks);
+    float top = -INFINITY;
+    auto vis = [&](int u, int i) {
+      return ((mine >> u) & 1u) && kv_sees(at.pos, p0 + u * kTile + i, a.window, a.sinks);
+    };
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!vis(p0 + v_pos(t, i))) {
-          if constexpr (BITS == 16)
-            vx.v[i][0] = vx.v[i][1] = make_uint4(0u, 0u, 0u, 0u);
-          else
-            vx.vs[i] = make_uint2(0u, 0u);
-        }
+    for (int u = 0; u < TILES; ++u) {
+      s[u][0] *= by;
+      s[u][1] *= by;
+      if (!full) {
+        if (!vis(u, g)) s[u][0] = -INFINITY;
+        if (!vis(u, g + 8)) s[u][1] = -INFINITY;
+      }
+      top = fmaxf(top, fmaxf(s[u][0], s[u][1]));
     }
-    float top = fmaxf(s[0], s[1]);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (__any_sync(0xffffffffu, top > acc.m)) {
@@ -531,20 +569,40 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
         for (int k = 0; k < 4; ++k) acc.o[i][k] *= f;
     }
     const float ref = acc.m == -INFINITY ? 0.f : acc.m;
-    const float w0 = exp2_fast((s[0] - ref) * 1.4426950408889634f);
-    const float w1 = exp2_fast((s[1] - ref) * 1.4426950408889634f);
-    acc.l += w0 + w1;
-    // weights of (positions v_pos(t, i); head g / 2): from the lanes that hold
-    // them as (position g' or g' + 8, head t')
-    float w[4];
-    const int src = 4 * t + (g >> 1);
-    w[0] = __shfl_sync(0xffffffffu, w0, src);
-    w[1] = __shfl_sync(0xffffffffu, w0, src + 16);
-    w[2] = __shfl_sync(0xffffffffu, w1, src);
-    w[3] = __shfl_sync(0xffffffffu, w1, src + 16);
-    acc.values(vx, w);
-    if constexpr (BITS == 16) {
-      if (it + 1 < steps) load_values(vx, cur + v_off);
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) {
+      const float w0 = exp2_fast((s[u][0] - ref) * 1.4426950408889634f);
+      const float w1 = exp2_fast((s[u][1] - ref) * 1.4426950408889634f);
+      acc.l += w0 + w1;
+      // weights of (positions v_pos(t, i); head g / 2): from the lanes that hold
+      // them as (position g' or g' + 8, head t')
+      float w[4];
+      const int src = 4 * t + (g >> 1);
+      w[0] = __shfl_sync(0xffffffffu, w0, src);
+      w[1] = __shfl_sync(0xffffffffu, w0, src + 16);
+      w[2] = __shfl_sync(0xffffffffu, w1, src);
+      w[3] = __shfl_sync(0xffffffffu, w1, src + 16);
+      // fp16 weights have one part: the odd columns are zero
+      if (Query<BITS, F32>::kHalf && plain && (g & 1)) w[0] = w[1] = w[2] = w[3] = 0.f;
+      if constexpr (BITS == 4) load_values(vx, p, u * kTile);
+      if (!full) {
+        // what a masked row holds must not meet its zero weight: it may be NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!vis(u, v_pos(t, i))) {
+            if constexpr (BITS == 16)
+              vx.v[i][0] = vx.v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            else
+              vx.vs[i] = make_uint2(0u, 0u);
+          }
+      }
+      acc.values(vx, w, plain);
+    }
+    if constexpr (BITS == 4) {
+      __syncwarp();  // every lane is done with the slot: it may be filled again
+      if (it + kRing < steps) start(it + kRing);
+    } else if (it + 1 < steps) {
+      load_values(vx, cur + v_off);
     }
   }
 
@@ -618,6 +676,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
 template <int BITS, bool F32>
 cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream_t stream) {
   auto kernel = k_kv_step<BITS, F32>;
+  constexpr int smem = BITS == 4 ? kStepWarps * kRing * (int)sizeof(Packed) : 0;
+  constexpr int UNIT = BITS == 4 ? kUnit : kTile;
   // clusters of 16 are past the portable size: asked for once per device
   static std::mutex mu;
   static bool ready[64] = {};
@@ -630,20 +690,22 @@ cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream
     if (!ready[dev]) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return e;
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
       ready[dev] = true;
     }
   }
   const int group = a.q_heads / c.g.kv_heads;
   const int chunks = (group + kStepHeads - 1) / kStepHeads;
   // How many CTAs share a row's positions: the least time by a model of waves,
-  // each a fixed part (3 us: tables, first loads, merging) and a part per tile
+  // each a fixed part (3 us: tables, first loads, merging) and a part per unit
   // of a warp (0.5 us with every warp of the SM at work). More CTAs shorten a
-  // wave and may add one; fewer than a tile per warp is never worth it.
+  // wave and may add one; fewer than a unit per warp is never worth it.
   const long long units = (long long)r.rows * c.g.kv_heads * chunks;
   long long longest = kv_capacity(c.g);
   if (r.max_length) longest = std::min<long long>(longest, r.max_length);
-  if (a.window) longest = std::min<long long>(longest, (long long)a.window + a.sinks + 2 * kTile);
-  const long long tiles = (longest + kTile - 1) / kTile, slots = 148LL * kStepCtas<BITS, F32>;
+  if (a.window) longest = std::min<long long>(longest, (long long)a.window + a.sinks + 2 * UNIT);
+  const long long tiles = (longest + UNIT - 1) / UNIT, slots = 148LL * kStepCtas<BITS, F32>;
   int ctas = 1;
   double best = 1e300;
   for (int n = 1; n <= kMaxCluster; n *= 2) {
@@ -659,6 +721,7 @@ cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(r.rows * (long long)ctas), (unsigned)(c.g.kv_heads * chunks));
   cfg.blockDim = dim3(kStepThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
