@@ -37,6 +37,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "common.cuh"
@@ -85,9 +86,11 @@ __device__ __forceinline__ void mma16816_half(float (&c)[4], const uint32_t (&a)
 __device__ __forceinline__ uint32_t shifted(uint32_t w, int left) {
   return left >= 0 ? w << left : w >> -left;
 }
-// Nibble i of each 16-bit half of w as the fp16 64 + code (mantissa bits 4-7).
+// Nibble i of each 16-bit half of w as the fp16 64 + code (mantissa bits 4-7):
+// one right shift serves two of them, the left shifts are products.
 __device__ __forceinline__ uint32_t nibbles_64(uint32_t w, int i) {
-  return (shifted(w, 4 - 4 * i) & 0x00f000f0u) | 0x54005400u;
+  const uint32_t x = i >= 2 ? w >> 8 : w;
+  return ((i & 1 ? x : x * 16u) & 0x00f000f0u) | 0x54005400u;
 }
 // As code - 8, exact, in fp16 or bf16 (there from 16 + code, mantissa bits 3-6).
 __device__ __forceinline__ uint32_t nibbles_half(uint32_t w, int i) {
@@ -697,22 +700,25 @@ cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream
   }
   const int group = a.q_heads / c.g.kv_heads;
   const int chunks = (group + kStepHeads - 1) / kStepHeads;
-  // How many CTAs share a row's positions: the least time by a model of waves,
-  // each a fixed part (3 us: tables, first loads, merging) and a part per unit
-  // of a warp (0.5 us with every warp of the SM at work). More CTAs shorten a
-  // wave and may add one; fewer than a unit per warp is never worth it.
-  const long long units = (long long)r.rows * c.g.kv_heads * chunks;
+  // How many CTAs share a row's positions: the least time by a model. The
+  // busiest SM works through ceil(units * n / 148) CTAs, a unit of a warp taking
+  // it 0.06 us when enough warps are at work, and 3 us go by for each wave (tables,
+  // first loads, merging); a warp alone takes 0.7 us a unit. More CTAs level the
+  // SMs and shorten lonely warps; fewer than a unit per warp is never worth it.
+  const long long rows_heads = (long long)r.rows * c.g.kv_heads * chunks;
   long long longest = kv_capacity(c.g);
   if (r.max_length) longest = std::min<long long>(longest, r.max_length);
   if (a.window) longest = std::min<long long>(longest, (long long)a.window + a.sinks + 2 * UNIT);
-  const long long tiles = (longest + UNIT - 1) / UNIT, slots = 148LL * kStepCtas<BITS, F32>;
+  const long long units = (longest + UNIT - 1) / UNIT;
   int ctas = 1;
   double best = 1e300;
   for (int n = 1; n <= kMaxCluster; n *= 2) {
-    if (n > 1 && tiles <= (long long)kStepWarps * (n / 2)) break;
-    const double waves = (double)((units * n + slots - 1) / slots);
-    const double per_warp = (double)((tiles + (long long)n * kStepWarps - 1) / (n * kStepWarps));
-    const double us = waves * (3.0 + 0.5 * per_warp);
+    if (n > 1 && units <= (long long)kStepWarps * (n / 2)) break;
+    const double busiest = (double)((rows_heads * n + 147) / 148);
+    const double waves = std::ceil(busiest / kStepCtas<BITS, F32>);
+    const double per_warp = (double)((units + (long long)n * kStepWarps - 1) / (n * kStepWarps));
+    const double us = 3.0 * waves + std::max(0.7 * per_warp * waves,
+                                             0.06 * kStepWarps * per_warp * busiest);
     if (us < best) {
       best = us;
       ctas = n;
