@@ -26,10 +26,10 @@
 //   fp16 (2^-12): scales past 2^12, or all below 2^-11, take the form below.
 //   fp32 rows: code - 8 in bf16 (exact), weight times scale in three parts.
 //
-// 16-bit tiles come into registers, refilled in place: the next K while its
-// weights meet V, the next V while its K is scored. 4-bit rows come 32 at a time
-// (four contiguous pieces, 4,608 bytes) by bulk copies into a ring of each
-// warp's own.
+// Rows come by bulk copies into a ring of each warp's own: 16 positions of 16
+// bits (two contiguous pieces of 4 KB) or 32 of 4 bits (four pieces, 4,608
+// bytes) to a slot. What is in flight does not depend on registers or on how
+// many warps an SM holds, which matters most for a few streams.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
 // CTAs of a cluster through distributed shared memory, both in a fixed order.
@@ -50,7 +50,6 @@ namespace {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = kStepWarps * 32;
 constexpr int kStepHeads = 4;   // query heads of one CTA
-constexpr int kRing = 2;        // 4-bit units of 32 positions in flight per warp
 constexpr int kTile = 16;       // positions of one matrix instruction; a page is a multiple
 constexpr int kMaxCluster = 16;
 constexpr long long kStepWaitCycles = 4000000000ll;  // two seconds at 2 GHz
@@ -134,32 +133,39 @@ struct Values<4> {
 // of a 4-bit tile at two to a bank.
 __device__ __forceinline__ int v_pos(int t, int i) { return t + 4 * i; }
 
-// A 4-bit unit in shared memory.
-constexpr int kUnit = 2 * kTile;
-struct __align__(16) Packed {
-  uint4 k[kUnit * 4], v[kUnit * 4];  // 64 bytes a row
-  uint2 ks[kUnit], vs[kUnit];
+// A slot of a warp's ring: `unit` positions of the cache, as they lie there.
+template <int BITS>
+struct Slot;
+template <>
+struct __align__(16) Slot<16> {
+  static constexpr int unit = kTile, ring = 3;
+  uint4 k[unit * 16], v[unit * 16];  // 256 bytes a row
+};
+template <>
+struct __align__(16) Slot<4> {
+  static constexpr int unit = 2 * kTile, ring = 2;
+  uint4 k[unit * 4], v[unit * 4];  // 64 bytes a row
+  uint2 ks[unit], vs[unit];
 };
 
-// 16 bits: rows of a K (V) tile from global memory.
-__device__ __forceinline__ void load_keys(Keys<16>& x, const unsigned char* rows) {
+// Operand fragments of the tile at row0 of a slot. (16-bit rows lie 256 bytes
+// apart, so lanes of neighbouring rows meet in a bank: twice the cycles for K and
+// four times for V, 192 a tile, where its 8 KB take an SM 350 at full rate.)
+__device__ __forceinline__ void load_keys(Keys<16>& x, const Slot<16>& p, int) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x.k[r][j] = __ldcg(reinterpret_cast<const uint4*>(rows + (g + 8 * r) * 256) + 4 * j + t);
+    for (int j = 0; j < 4; ++j) x.k[r][j] = p.k[(g + 8 * r) * 16 + 4 * j + t];
 }
-__device__ __forceinline__ void load_values(Values<16>& x, const unsigned char* rows) {
+__device__ __forceinline__ void load_values(Values<16>& x, const Slot<16>& p, int) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      x.v[i][h] = __ldcg(reinterpret_cast<const uint4*>(rows + v_pos(t, i) * 256) + 8 * h + g);
+    for (int h = 0; h < 2; ++h) x.v[i][h] = p.v[v_pos(t, i) * 16 + 8 * h + g];
 }
-// 4 bits: from the ring.
-__device__ __forceinline__ void load_keys(Keys<4>& x, const Packed& p, int row0) {
+__device__ __forceinline__ void load_keys(Keys<4>& x, const Slot<4>& p, int row0) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -167,7 +173,7 @@ __device__ __forceinline__ void load_keys(Keys<4>& x, const Packed& p, int row0)
     x.ks[r] = p.ks[row0 + g + 8 * r];
   }
 }
-__device__ __forceinline__ void load_values(Values<4>& x, const Packed& p, int row0) {
+__device__ __forceinline__ void load_values(Values<4>& x, const Slot<4>& p, int row0) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -401,17 +407,19 @@ struct Partial {
   float o[kStepHeads][kKvDim];
 };
 
-// CTAs on an SM: what the registers of the form allow.
+// CTAs on an SM: what registers (4 bits) or rings (16 bits) allow.
 template <int BITS, bool F32>
-constexpr int kStepCtas = BITS == 4 && !F32 ? 4 : 3;
+constexpr int kStepCtas = BITS == 16 ? 2 : F32 ? 3 : 4;
 
 template <int BITS, bool F32>
 __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
     k_kv_step(KvArgs c, KvRows r, KvAttend a, int chunks) {
   __shared__ Partial s_warp[kStepWarps];
   __shared__ Partial s_cta;
-  extern __shared__ Packed s_rings[];  // 4 bits: kRing per warp
-  __shared__ uint64_t s_full[kStepWarps][kRing];
+  using Sl = Slot<BITS>;
+  constexpr int RING = Sl::ring, UNIT = Sl::unit, TILES = UNIT / kTile;
+  extern __shared__ uint4 s_rings[];
+  __shared__ uint64_t s_full[kStepWarps][RING];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -426,8 +434,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
   Query<BITS, F32> q;
   load_query<BITS, F32>(q, a.q.p, (long long)row * a.q.row + (long long)(qh0 + (g >> 1)) * a.q.head,
                         (g >> 1) < heads);
-  // visible units (of 16 positions, 32 for 4 bits): [0, ns) and [ws, pos / unit]
-  constexpr int TILES = BITS == 4 ? 2 : 1, UNIT = TILES * kTile;
+  // visible units: [0, ns) and [ws, pos / UNIT]
   const KvSpan sp = kv_span(at.ok ? at.pos : 0, a.window, a.sinks);
   const int ns = (sp.sink_end + UNIT - 1) / UNIT;
   const int ws = max(sp.first / UNIT, ns);
@@ -459,86 +466,70 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
     const int p = un * UNIT + lane % TILES * kTile;
     pages = un >= 0 && p <= at.pos ? kv_page(c, at.seq, p >> c.g.shift) : -1;
   };
-  Keys<BITS> kx;
-  Values<BITS> vx;
-  const unsigned char* cur = kbase;
-  unsigned has = 0u;  // which tiles of a step have a page: TILES bits per ring slot
+  unsigned has = 0u;  // which tiles of a unit have a page: TILES bits per slot
   constexpr unsigned ALL = (1u << TILES) - 1u;
-  auto rows_of = [&](int it) {  // 16 bits
+  Sl* ring = reinterpret_cast<Sl*>(s_rings) + warp * RING;
+  const int piece = min(mask + 1, UNIT);  // rows of a unit that lie in one page
+  // starts the copies of step it's unit
+  auto start = [&](int it, int slot) {
     if (it % HELD == 0) refill(it);
-    const int page = __shfl_sync(0xffffffffu, pages, it % HELD);
-    has = page >= 0;
-    return kbase + max(page, 0) * page_bytes + ((unit_of(it) * UNIT) & mask) * (2 * kKvDim);
-  };
-  // 4 bits: starts the copies of step it's unit, in one piece if a page holds it
-  static_assert((kRing & (kRing - 1)) == 0, "slots by masking");
-  Packed* ring = s_rings + warp * kRing;
-  const int piece = min(mask + 1, kUnit), scales = kKvCodeBytes << c.g.shift;
-  auto start = [&](int it) {
-    if (it % HELD == 0) refill(it);
-    const int slot = it & (kRing - 1), bit = it % HELD * TILES;
+    const int bit = it % HELD * TILES;
     const int pg0 = __shfl_sync(0xffffffffu, pages, bit);
-    const int pg1 = __shfl_sync(0xffffffffu, pages, bit + TILES - 1);
-    has = (has & ~(ALL << (slot * TILES))) | ((pg0 >= 0) | (pg1 >= 0) << 1) << (slot * TILES);
+    const int pg1 = TILES > 1 ? __shfl_sync(0xffffffffu, pages, bit + 1) : 0;
+    has = (has & ~(ALL << (slot * TILES))) |
+          ((pg0 >= 0) | (TILES > 1 && pg1 >= 0) << 1) << (slot * TILES);
     if (lane == 0) {
-      Packed& p = ring[slot];
+      Sl& p = ring[slot];
       uint64_t* bar = &s_full[warp][slot];
-      mbar_expect_tx(bar, sizeof(Packed));
+      mbar_expect_tx(bar, sizeof(Sl));
       const int row = (unit_of(it) * UNIT) & mask;
-      for (int u = 0; u < kUnit; u += piece) {  // pieces of 16 start a page
-        const unsigned char* tile = kbase + max(u ? pg1 : pg0, 0) * page_bytes;
-        const unsigned char* k = tile + row * kKvCodeBytes;
-        const unsigned char* ks = tile + scales + row * 2 * kKvGroups;
-        bulk_g2s(p.k + 4 * u, k, piece * kKvCodeBytes, bar);
-        bulk_g2s(p.ks + u, ks, piece * 2 * kKvGroups, bar);
-        bulk_g2s(p.v + 4 * u, k + v_off, piece * kKvCodeBytes, bar);
-        bulk_g2s(p.vs + u, ks + v_off, piece * 2 * kKvGroups, bar);
+      if constexpr (BITS == 16) {
+        const unsigned char* k = kbase + max(pg0, 0) * page_bytes + row * (2 * kKvDim);
+        bulk_g2s(p.k, k, sizeof p.k, bar);
+        bulk_g2s(p.v, k + v_off, sizeof p.v, bar);
+      } else {
+        for (int u = 0; u < UNIT; u += piece) {  // pieces of 16 start a page
+          const unsigned char* tile = kbase + max(u ? pg1 : pg0, 0) * page_bytes;
+          const unsigned char* k = tile + row * kKvCodeBytes;
+          const unsigned char* ks = tile + (kKvCodeBytes << c.g.shift) + row * 2 * kKvGroups;
+          bulk_g2s(p.k + 4 * u, k, piece * kKvCodeBytes, bar);
+          bulk_g2s(p.ks + u, ks, piece * 2 * kKvGroups, bar);
+          bulk_g2s(p.v + 4 * u, k + v_off, piece * kKvCodeBytes, bar);
+          bulk_g2s(p.vs + u, ks + v_off, piece * 2 * kKvGroups, bar);
+        }
       }
     }
   };
-  if constexpr (BITS == 4) {
-    if (lane == 0)
-      for (int i = 0; i < kRing; ++i) mbar_init(&s_full[warp][i], 1);
-    fence_mbar_init();
-    __syncwarp();
-    for (int i = 0; i < kRing && i < steps; ++i) start(i);
-  } else if (steps) {
-    cur = rows_of(0);
-    load_keys(kx, cur);
-    load_values(vx, cur + v_off);
-  }
+  if (lane == 0)
+    for (int i = 0; i < RING; ++i) mbar_init(&s_full[warp][i], 1);
+  fence_mbar_init();
+  __syncwarp();
+  for (int i = 0; i < RING && i < steps; ++i) start(i, i);
+  int slot = 0, phase = 0;
   for (int it = 0; it < steps; ++it) {
-    float s[TILES][2];
-    const int slot = it & (kRing - 1);
-    const unsigned mine = BITS == 4 ? has >> (slot * TILES) & ALL : has;
-    const Packed& p = ring[slot];
+    const unsigned mine = has >> (slot * TILES) & ALL;
+    const Sl& p = ring[slot];
+    const bool landed = mbar_wait_cycles(&s_full[warp][slot], phase, kStepWaitCycles);
+    if (!__all_sync(0xffffffffu, landed)) {
+      kv_status(c, kKvTimeout);
+      for (int i = 0; i < RING; ++i)  // no copy may outlive the CTA
+        if (i != slot) mbar_wait_cycles(&s_full[warp][i], i > slot ? phase : phase ^ 1, kStepWaitCycles);
+      break;
+    }
     bool plain = true;
-    if constexpr (BITS == 4) {
-      const bool landed = mbar_wait_cycles(&s_full[warp][slot], (it / kRing) & 1, kStepWaitCycles);
-      if (!__all_sync(0xffffffffu, landed)) {
-        kv_status(c, kKvTimeout);
-        for (int i = it + 1; i < min(it + kRing, steps); ++i)  // no copy may outlive the CTA
-          mbar_wait_cycles(&s_full[warp][i % kRing], (i / kRing) & 1, kStepWaitCycles);
-        break;
-      }
-      if constexpr (!F32) {
-        // the four scales of V's row `lane` (bf16 bits): past 2^12, not a number or
-        // negative; or all below 2^-11, where fp16's multiples of 2^-24 begin to show
-        const uint2 vs = p.vs[lane];
-        const unsigned top = max(max(vs.x & 0xffffu, vs.x >> 16), max(vs.y & 0xffffu, vs.y >> 16));
-        plain = !__any_sync(0xffffffffu, top > 0x4580u || (top != 0u && top < 0x3a00u));
-      }
+    if constexpr (Query<BITS, F32>::kHalf) {
+      // the four scales of V's row `lane` (bf16 bits): past 2^12, not a number or
+      // negative; or all below 2^-11, where fp16's multiples of 2^-24 begin to show
+      const uint2 vs = p.vs[lane];
+      const unsigned top = max(max(vs.x & 0xffffu, vs.x >> 16), max(vs.y & 0xffffu, vs.y >> 16));
+      plain = !__any_sync(0xffffffffu, top > 0x4580u || (top != 0u && top < 0x3a00u));
+    }
+    float s[TILES][2];
 #pragma unroll
-      for (int u = 0; u < TILES; ++u) {
-        load_keys(kx, p, u * kTile);
-        acc.scores(kx, q, s[u][0], s[u][1]);
-      }
-    } else {
-      acc.scores(kx, q, s[0][0], s[0][1]);
-      if (it + 1 < steps) {
-        cur = rows_of(it + 1);
-        load_keys(kx, cur);
-      }
+    for (int u = 0; u < TILES; ++u) {
+      Keys<BITS> kx;
+      load_keys(kx, p, u * kTile);
+      acc.scores(kx, q, s[u][0], s[u][1]);
     }
     const float by = a.scale * q.unscale;
     const int p0 = unit_of(it) * UNIT;
@@ -587,7 +578,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
       w[3] = __shfl_sync(0xffffffffu, w1, src + 16);
       // fp16 weights have one part: the odd columns are zero
       if (Query<BITS, F32>::kHalf && plain && (g & 1)) w[0] = w[1] = w[2] = w[3] = 0.f;
-      if constexpr (BITS == 4) load_values(vx, p, u * kTile);
+      Values<BITS> vx;
+      load_values(vx, p, u * kTile);
       if (!full) {
         // what a masked row holds must not meet its zero weight: it may be NaN
 #pragma unroll
@@ -601,11 +593,11 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
       }
       acc.values(vx, w, plain);
     }
-    if constexpr (BITS == 4) {
-      __syncwarp();  // every lane is done with the slot: it may be filled again
-      if (it + kRing < steps) start(it + kRing);
-    } else if (it + 1 < steps) {
-      load_values(vx, cur + v_off);
+    __syncwarp();  // every lane is done with the slot: it may be filled again
+    if (it + RING < steps) start(it + RING, slot);
+    if (++slot == RING) {
+      slot = 0;
+      phase ^= 1;
     }
   }
 
@@ -679,8 +671,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
 template <int BITS, bool F32>
 cudaError_t step(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream_t stream) {
   auto kernel = k_kv_step<BITS, F32>;
-  constexpr int smem = BITS == 4 ? kStepWarps * kRing * (int)sizeof(Packed) : 0;
-  constexpr int UNIT = BITS == 4 ? kUnit : kTile;
+  constexpr int smem = kStepWarps * Slot<BITS>::ring * (int)sizeof(Slot<BITS>);
+  constexpr int UNIT = Slot<BITS>::unit;
   // clusters of 16 are past the portable size: asked for once per device
   static std::mutex mu;
   static bool ready[64] = {};
