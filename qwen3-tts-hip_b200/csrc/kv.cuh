@@ -122,24 +122,44 @@ __device__ __forceinline__ float4 kv_cached4(const KvArgs& c, int page, int laye
                      (float)((int)((n >> 8) & 15u) - 8) * s, (float)((int)(n >> 12) - 8) * s);
 }
 
+__device__ __forceinline__ void kv_load8(const void* p, long long off, int type, float (&x)[8]) {
+  const float4 a = kv_load4(p, off, type), b = kv_load4(p, off + 4, type);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void kv_store8(void* p, long long off, int type, const float (&x)[8]) {
+  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p) + off;
+  if (type == KV_BF16 && (reinterpret_cast<uintptr_t>(h) & 15) == 0) {
+    __nv_bfloat162 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(w);
+    return;
+  }
+  kv_store4(p, off, type, make_float4(x[0], x[1], x[2], x[3]));
+  kv_store4(p, off + 4, type, make_float4(x[4], x[5], x[6], x[7]));
+}
+
 // Scale of a group from its largest magnitude: amax / 7 rounded once to the
-// nearest bf16 (ties to even). fl(amax / 7) may sit on a bf16 midpoint that
-// the exact quotient only comes near, so the midpoint decides by 7 * mid,
-// which is exact (12 bits). Non-finite: NaN, which marks the group.
+// nearest bf16 (ties to even). The fp32 quotient q (an ulp or two off) is only
+// used to find the bf16 values s0 <= q and s1 around the exact quotient, or s0
+// one step high where q reached a value that the exact quotient just misses;
+// in every case the midpoint decides: amax against 7 * mid, which is exact (12
+// bits). Non-finite: NaN, which marks the group.
 __device__ __forceinline__ float kv_scale_of(float amax) {
   if (!isfinite(amax)) return __int_as_float(0x7fc00000);
-  const unsigned lo = __float_as_uint(amax / 7.0f) & 0xffff0000u;
+  const unsigned lo = __float_as_uint(amax * (1.0f / 7.0f)) & 0xffff0000u;
   const float s0 = __uint_as_float(lo), s1 = __uint_as_float(lo + 0x10000u);
   const float mid7 = 7.0f * (s0 + 0.5f * (s1 - s0));
   return amax > mid7 || (amax == mid7 && (lo & 0x10000u)) ? s1 : s0;
 }
 // Code of x: x / s rounded once to the nearest integer (ties to even), limited
-// to -7..7, plus 8. The rounded quotient may sit on a half the exact one does
-// not reach, so (n +- 1/2) * s, exact in fp32 (13 bits), decides.
-__device__ __forceinline__ unsigned kv_code_of(float x, float s) {
-  if (!(s > 0.f)) return 8u;  // all zeros, or a marked group
+// to -7..7, plus 8. x * inv is at most one off after rounding; (n +- 1/2) * s,
+// exact in fp32 (13 bits), decides. inv: 1 / s, or infinity for subnormal s,
+// where the quotient itself is taken.
+__device__ __forceinline__ unsigned kv_code_of(float x, float s, float inv) {
   const float a = fabsf(x);
-  float n = fminf(rintf(a / s), 8.0f);
+  float n = fminf(rintf(inv < 3e38f ? a * inv : a / s), 8.0f);
   const float up = (n + 0.5f) * s, dn = (n - 0.5f) * s;
   const bool odd = ((int)n & 1) != 0;
   if (a > up || (a == up && odd)) n += 1.0f;
@@ -147,18 +167,25 @@ __device__ __forceinline__ unsigned kv_code_of(float x, float s) {
   n = fminf(n, 7.0f);
   return (unsigned)(8 + (int)(x < 0.f ? -n : n));
 }
-// Warp-collective over the eight lanes of a group: the 16 bits of this lane's
-// four codes, and the group's scale.
-__device__ __forceinline__ unsigned kv_quantise4(float4 x, float* scale) {
+// Warp-collective over the four lanes of a group: this lane's eight codes, and
+// the group's scale.
+__device__ __forceinline__ uint32_t kv_quantise8(const float (&x)[8], float* scale) {
   // a NaN would drop out of fmaxf: it is carried as infinity
-  auto mag = [](float v) { return v == v ? fabsf(v) : __int_as_float(0x7f800000); };
-  float m = fmaxf(fmaxf(mag(x.x), mag(x.y)), fmaxf(mag(x.z), mag(x.w)));
+  float m = 0.f;
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int d = 0; d < 8; ++d) m = fmaxf(m, x[d] == x[d] ? fabsf(x[d]) : __int_as_float(0x7f800000));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const float s = kv_scale_of(m);
   *scale = s;
-  return kv_code_of(x.x, s) | (kv_code_of(x.y, s) << 4) | (kv_code_of(x.z, s) << 8) |
-         (kv_code_of(x.w, s) << 12);
+  uint32_t w = 0x88888888u;
+  if (s > 0.f) {  // else all zeros, or a marked group
+    const float inv = s >= 1.1754944e-38f ? 1.0f / s : __int_as_float(0x7f800000);
+    w = 0u;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) w |= kv_code_of(x[d], s, inv) << (4 * d);
+  }
+  return w;
 }
 
 // One (row, q head) by one warp, position by position, eight at a time: a

@@ -8,72 +8,111 @@ namespace qtts {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kRowBatch = 4;  // pairs of units in flight per warp
 
-// One warp per (row, K or V, kv head); lane l holds dims 4 l .. 4 l + 3, so
-// eight lanes share a group's scale. Every byte is touched once: the rows in,
-// the codes and scales out.
+// A unit is one row of K or V of one kv head; a half-warp takes it, lane l of it
+// dims 8 l .. 8 l + 7 (one word of codes; four lanes share a scale). A warp has
+// one row's place and up to eight of its units, whose values are on their way
+// while the place is looked up (three dependent reads). Bound by bytes: every
+// value is read once and written once.
 template <bool READ>
 __global__ void __launch_bounds__(kRowThreads)
-    k_kv_rows(KvArgs c, KvRows r, int layer, KvTensor k, KvTensor v, int type) {
+    k_kv_rows(KvArgs c, KvRows r, int layer, KvTensor k, KvTensor v, int type, int per_row) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const long long unit = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
-  const int per = 2 * c.g.kv_heads;
-  const int row = (int)(unit / per), u = (int)(unit - (long long)row * per);
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const long long warp = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
+  const int row = (int)(warp / per_row);
   if (row >= r.rows) return;
-  const int which = u / c.g.kv_heads, head = u - which * c.g.kv_heads;
+  const int units = 2 * c.g.kv_heads;
+  const int u0 = (int)(warp - (long long)row * per_row) * 2 * kRowBatch + (lane >> 4);
+  auto tensor_at = [&](int u, long long* off) -> const KvTensor& {
+    const bool is_v = u >= c.g.kv_heads;
+    const KvTensor& t = is_v ? v : k;
+    *off = (long long)row * t.row + (long long)(is_v ? u - c.g.kv_heads : u) * t.head + 8 * l;
+    return t;
+  };
+  float x[kRowBatch][8];
+  if (!READ) {
+#pragma unroll
+    for (int i = 0; i < kRowBatch; ++i)
+      if (u0 + 2 * i < units) {
+        long long off;
+        const KvTensor& t = tensor_at(u0 + 2 * i, &off);
+        kv_load8(t.p, off, type, x[i]);
+      }
+  }
   const KvPlace at = kv_place(c, r, row, !READ);
   if (at.group < 0) return;
-  const KvTensor& t = which ? v : k;
-  const long long off = (long long)row * t.row + (long long)head * t.head + 4 * lane;
   const int page = at.ok ? kv_page(c, at.seq, at.pos >> c.g.shift) : -1;
-  if (page < 0) {
-    // nothing is held there: nothing is written, and a row read is zeros
-    if (READ) kv_store4(t.p, off, type, make_float4(0.f, 0.f, 0.f, 0.f));
-    else if (at.ok) kv_bad(c);
+  if (!READ && page < 0) {  // nothing to write into
+    if (at.ok) kv_bad(c);
     return;
   }
   const int prow = at.pos & ((1 << c.g.shift) - 1);
-  unsigned char* tile = c.pool + kv_tile_at(c.g, page, layer, which, head);
-  unsigned char* cell = tile + kv_row_at(c.g, prow);
-  if (c.g.bits == 16) {
-    uint2* w = reinterpret_cast<uint2*>(cell) + lane;
-    if (READ) {
-      const uint2 x = *w;
-      kv_store4(t.p, off, type,
-                make_float4(bf16lo(x.x), bf16hi(x.x), bf16lo(x.y), bf16hi(x.y)));
-    } else {
-      const float4 x = kv_load4(t.p, off, type);
-      const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-      *w = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+  // the K tiles of all heads, then the V tiles, follow one another
+  const long long tile = kv_tile_bytes(c.g);
+  unsigned char* base = c.pool + kv_tile_at(c.g, max(page, 0), layer, 0, 0);
+  uint4 w[kRowBatch];
+  uint32_t sc[kRowBatch];
+  if (READ && page >= 0) {
+#pragma unroll
+    for (int i = 0; i < kRowBatch; ++i) {
+      if (u0 + 2 * i >= units) continue;
+      const unsigned char* t = base + (u0 + 2 * i) * tile;
+      if (c.g.bits == 16) {
+        w[i] = __ldcg(reinterpret_cast<const uint4*>(t + prow * 2 * kKvDim) + l);
+      } else {
+        w[i].x = __ldcg(reinterpret_cast<const uint32_t*>(t + prow * kKvCodeBytes + kv_code_word_at(8 * l)));
+        sc[i] = __ldcg(reinterpret_cast<const uint16_t*>(t + kv_scale_at(c.g, prow)) + (l >> 2));
+      }
     }
-    return;
   }
-  uint16_t* code = reinterpret_cast<uint16_t*>(cell + kv_code_word_at(4 * lane)) + (lane & 1);
-  __nv_bfloat16* sc = reinterpret_cast<__nv_bfloat16*>(tile + kv_scale_at(c.g, prow)) + (lane >> 3);
-  if (READ) {
-    const unsigned n = *code;
-    const float s = __bfloat162float(*sc);
-    kv_store4(t.p, off, type,
-              make_float4((float)((int)(n & 15u) - 8) * s, (float)((int)((n >> 4) & 15u) - 8) * s,
-                          (float)((int)((n >> 8) & 15u) - 8) * s, (float)((int)(n >> 12) - 8) * s));
-    return;
+#pragma unroll
+  for (int i = 0; i < kRowBatch; ++i) {
+    const bool in = u0 + 2 * i < units;  // uniform in a half-warp
+    if (READ) {
+      if (!in) continue;
+      float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // no page: zeros
+      if (page >= 0 && c.g.bits == 16) {
+        unpack8(w[i], y);
+      } else if (page >= 0) {
+        const float s = __uint_as_float(sc[i] << 16);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[d] = (float)((int)((w[i].x >> (4 * d)) & 15u) - 8) * s;
+      }
+      long long off;
+      const KvTensor& t = tensor_at(u0 + 2 * i, &off);
+      kv_store8(t.p, off, type, y);
+      continue;
+    }
+    unsigned char* t = base + (u0 + 2 * i) * tile;
+    if (c.g.bits == 16) {
+      if (!in) continue;
+      float y[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) y[d] = x[i][d];
+      kv_store8(t + prow * 2 * kKvDim, 8 * l, KV_BF16, y);
+      continue;
+    }
+    // the lanes of a unit that is not there take part in the shuffles
+    float s;
+    const uint32_t codes = kv_quantise8(x[i], &s);
+    if (!in) continue;
+    *reinterpret_cast<uint32_t*>(t + prow * kKvCodeBytes + kv_code_word_at(8 * l)) = codes;
+    if ((l & 3) == 0)
+      *(reinterpret_cast<__nv_bfloat16*>(t + kv_scale_at(c.g, prow)) + (l >> 2)) = __float2bfloat16_rn(s);
   }
-  const float4 x = kv_load4(t.p, off, type);
-  float s;
-  *code = (uint16_t)kv_quantise4(x, &s);
-  if ((lane & 7) == 0) *sc = __float2bfloat16_rn(s);
 }
 
 template <bool READ>
 cudaError_t rows_op(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                     const KvTensor& v, int type, cudaStream_t stream) {
-  const long long warps = (long long)r.rows * 2 * c.g.kv_heads;
-  if (warps == 0) return cudaSuccess;
-  const long long ctas = (warps * 32 + kRowThreads - 1) / kRowThreads;
+  if (r.rows == 0) return cudaSuccess;
+  const int per_row = (2 * c.g.kv_heads + 2 * kRowBatch - 1) / (2 * kRowBatch);
+  const long long ctas = ((long long)r.rows * per_row * 32 + kRowThreads - 1) / kRowThreads;
   return launch(k_kv_rows<READ>, dim3((unsigned)ctas), dim3(kRowThreads), 0, stream, c, r, layer, k,
-                v, type);
+                v, type, per_row);
 }
 
 }  // namespace

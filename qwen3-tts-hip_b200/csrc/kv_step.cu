@@ -294,18 +294,27 @@ struct Warp {
   __device__ __forceinline__ void scores(const Keys<BITS>& x, const Query<BITS, F32>& q, float& s0,
                                          float& s1) {
     if constexpr (BITS == 16) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      // fp32 rows, twice the products: four sums at once (one would wait for each
+      // product in turn: 22.9 instead of 23.5 us for 16 streams)
+      constexpr int SUMS = F32 ? 4 : 1;
+      float c[SUMS][4] = {};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int j = 0; j < 4; ++j) {
           const uint32_t a[4] = {word(x.k[0][j], 2 * s), word(x.k[1][j], 2 * s),
                                  word(x.k[0][j], 2 * s + 1), word(x.k[1][j], 2 * s + 1)};
-          mma16816(c, a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
-          if constexpr (F32) mma16816(c, a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
+          mma16816(c[j % SUMS], a, q.b[2 * j + s][0], q.b[2 * j + s][1]);
+          if constexpr (F32) mma16816(c[j % SUMS], a, q.b[2 * j + s][2], q.b[2 * j + s][3]);
         }
-      s0 = F32 ? c[0] + c[1] : c[0];
-      s1 = F32 ? c[2] + c[3] : c[2];
+      auto sum = [&](int i) {
+        float v = c[0][i];
+#pragma unroll
+        for (int k = 1; k < SUMS; ++k) v += c[k][i];
+        return v;
+      };
+      s0 = F32 ? sum(0) + sum(1) : sum(0);
+      s1 = F32 ? sum(2) + sum(3) : sum(2);
     } else {
       s0 = s1 = 0.f;
 #pragma unroll
