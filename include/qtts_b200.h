@@ -131,6 +131,24 @@ int32_t qtts_engine_load_with_max_frames(const char* model_dir, int32_t device,
 /* HipTtsEngine::load_with_options (generation.rs:284-315). */
 int32_t qtts_engine_load_with_options(const char* model_dir, int32_t device,
                                       size_t max_cache_steps, qtts_engine** out);
+/* The same with a choice of how the talker's cache is kept (no reference
+ * counterpart). kv_bits 4: keys and values in the 4-bit form described with
+ * qtts_kv_cache below, 72 bytes a row instead of 256. window > 0: a position
+ * sees the last `window` positions (itself included) and the first `sinks`,
+ * so a frame's attention costs the same however long the speech gets (the
+ * cache still holds every position). Both change what is generated, as any
+ * change of the attention does; with kv_bits 16 and window 0 the engine is
+ * that of qtts_engine_load_with_options. The CodePredictor's cache (16
+ * positions) stays as it is. */
+typedef struct {
+  size_t max_cache_steps; /* 512 */
+  int32_t kv_bits;        /* 16 or 4 */
+  int32_t window;         /* 0: every earlier position */
+  int32_t sinks;
+} qtts_cache_options;
+void qtts_cache_options_default(qtts_cache_options* out);
+int32_t qtts_engine_load_with_cache(const char* model_dir, int32_t device,
+                                    const qtts_cache_options* cache, qtts_engine** out);
 void qtts_engine_destroy(qtts_engine* engine);
 int32_t qtts_engine_get_info(const qtts_engine* engine, qtts_engine_info* out);
 
@@ -182,6 +200,17 @@ int32_t qtts_generate_codes_batch_from_ids(qtts_engine* engine, const uint32_t* 
                                            const qtts_generate_options* opts, int32_t* codes_out,
                                            size_t cap_per_request, size_t* frames_out,
                                            int32_t* ended_out);
+
+/* Several takes (1..16) of one prompt, seeds[t] in place of options->seed
+ * (no reference counterpart): what qtts_generate_codes_batch_from_ids gives for
+ * that many copies of the request, with the prompt prefilled once and its
+ * cache pages shared (qtts_kv_fork). Codes of take t go to
+ * codes_out + t * cap_per_take. */
+int32_t qtts_generate_codes_takes_from_ids(qtts_engine* engine, const uint32_t* content_ids,
+                                           size_t n_ids, const qtts_generate_options* options,
+                                           const uint64_t* seeds, size_t takes,
+                                           int32_t* codes_out, size_t cap_per_take,
+                                           size_t* frames_out, int32_t* ended_out);
 
 /* HipTtsEngine::generate_voice_clone_codes (generation.rs:373-395), x-vector
  * mode: speaker_embedding[hidden] replaces the speaker codec row

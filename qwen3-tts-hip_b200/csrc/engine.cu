@@ -34,6 +34,7 @@
 #include "gemm_tc.h"
 #include "json.h"
 #include "kernels.h"
+#include "kv.h"
 #include "qtts_b200.h"
 
 namespace qtts {
@@ -769,8 +770,19 @@ class Codec {
 
 class Engine {
  public:
-  Engine(const std::string& dir, int device, size_t max_cache_steps);
+  Engine(const std::string& dir, int device, const qtts_cache_options& cache);
   ~Engine();
+
+  // How the talker's cache is kept: bf16 with every position seen, by the fused
+  // decode and prefill attention of kernels.cu; or in 4 bits and / or seen
+  // through a window, by the kernels of kv_*.cu (kv_form).
+  const qtts_cache_options cache;
+  bool kv_form() const { return cache.kv_bits != 16 || cache.window != 0; }
+  int* kv_word = nullptr;  // their status
+  KvArgs kv_args(const KvView& kv, int seqs, int max_pages, const int* pos, int pos_stride, int pos0);
+  void kv_attention(DevStack& S, StackBufs& B, const KvArgs& c, const KvRows& r, int layer,
+                    const int* halt, int halt_stride);
+  void check_kv();
 
   ModelCfg cfg;
   size_t max_cache_steps;
@@ -844,6 +856,13 @@ class Engine {
   float* cp_qkv0 = nullptr;
   float* cp_x0 = nullptr;  // with the input projection: [groups-2][vocab][cp hidden] projected rows
   void build_cp_qkv_table();
+  // Talker pages in the cache's format (16 bits: page_stride elements each).
+  __nv_bfloat16* alloc_talker_pool(int pages) {
+    if (cache.kv_bits == 16) return arena.alloc<__nv_bfloat16>((size_t)(tkv.page_stride * pages));
+    const KvGeom g{1, 1, 1, cfg.talker.layers, cfg.talker.kv_heads, kTalkerPageShift, cache.kv_bits};
+    return reinterpret_cast<__nv_bfloat16*>(
+        arena.alloc<unsigned char>((size_t)kv_page_bytes(g) * pages));
+  }
   cudaEvent_t ev0 = nullptr, ev1 = nullptr, ev2 = nullptr;
   float last_prefill_ms = 0.f, last_frames_ms = 0.f;
   size_t last_frames = 0;
@@ -941,10 +960,14 @@ class Engine {
     StackBufs tb{}, cb{};
     KvView tkv{}, ckv{};
     int pages = 0;  // talker KV pages per sequence
+    // takes of one prompt: tables of their own over tkv's pages, filled by
+    // launch_kv_resize / launch_kv_fork, so that full prompt pages are shared
+    KvArgs takes{};
     TcPlan plan{};
     float* rms = nullptr;  // [cap] RMS scale of each head input row
     cudaEvent_t ev[3] = {nullptr, nullptr, nullptr};  // prefill start, frames start, end
   } bt;
+  // by sampling, sequences (negative: takes, on their own tables)
   std::map<std::pair<SampleKey, int>, cudaGraphExec_t> batch_graphs;
   std::map<std::pair<SampleKey, int>, size_t> batch_nodes;
   void ensure_batch();
@@ -954,8 +977,16 @@ class Engine {
   void batch_stack_step(DevStack& S, StackBufs& B, const KvView& kv, int pt_stride,
                         const int* pos_ptr, int pos_const, int nb, bool qkv0_given = false);
   void batch_head(int role, int group, const float* x, const SampleCfg& c, float penalty, int nb);
-  void enqueue_batch_frame(const SampleKey& k, int nb);
-  cudaGraphExec_t batch_graph(const SampleKey& k, int nb);
+  void enqueue_batch_frame(const SampleKey& k, int nb, const KvView& tkv);
+  cudaGraphExec_t batch_graph(const SampleKey& k, int nb, const KvView& tkv, bool takes);
+  void store_slot(int b, int ntr);
+  void run_batch(int nb, const qtts_generate_options& o, const KvView& view, bool takes,
+                 int32_t* codes_out, size_t cap_per_request, size_t* frames_out,
+                 int32_t* ended_out);
+  void ensure_takes();
+  void generate_takes(const uint32_t* ids, size_t n, const qtts_generate_options& o,
+                      const std::vector<uint64_t>& seeds, int32_t* codes_out,
+                      size_t cap_per_take, size_t* frames_out, int32_t* ended_out);
   void generate_batch(const std::vector<std::vector<uint32_t>>& ids,
                       const std::vector<qtts_generate_options>& opts, int32_t* codes_out,
                       size_t cap_per_request, size_t* frames_out, int32_t* ended_out);
@@ -1094,8 +1125,14 @@ StackBufs alloc_bufs(Arena& arena, const DevStack& S, int rows) {
   return b;
 }
 
-Engine::Engine(const std::string& dir, int dev, size_t mcs) : max_cache_steps(mcs), device(dev) {
+Engine::Engine(const std::string& dir, int dev, const qtts_cache_options& co)
+    : cache(co), max_cache_steps(co.max_cache_steps), device(dev) {
+  const size_t mcs = max_cache_steps;
   if (mcs == 0) invalid("max_cache_steps must be non-zero");
+  if (co.kv_bits != 16 && co.kv_bits != 4)
+    invalid("kv_bits must be 16 or 4, got " + std::to_string(co.kv_bits));
+  if (co.window < 0 || co.sinks < 0) invalid("window and sinks must not be negative");
+  if (co.sinks > 0 && co.window == 0) invalid("sinks need a window");
   cfg = load_config(dir);
   int ndev = 0;
   QCK(cudaGetDeviceCount(&ndev));
@@ -1198,7 +1235,7 @@ Engine::Engine(const std::string& dir, int dev, size_t mcs) : max_cache_steps(mc
     tkv.kv_heads = T.kv_heads;
     tkv.layer_stride = (long long)2 * T.kv_heads * (1 << shift) * kHeadDim;
     tkv.page_stride = tkv.layer_stride * T.layers;
-    tkv.pool = arena.alloc<__nv_bfloat16>((size_t)(tkv.page_stride * pages));
+    tkv.pool = alloc_talker_pool(pages);
     std::vector<int> pt(pages);
     for (int i = 0; i < pages; ++i) pt[i] = i;
     int* d = arena.alloc<int>(pages);
@@ -1215,6 +1252,7 @@ Engine::Engine(const std::string& dir, int dev, size_t mcs) : max_cache_steps(mc
     ckv.pool = arena.alloc<__nv_bfloat16>((size_t)ckv.page_stride);
     ckv.page_table = arena.alloc<int>(1);  // one entry: page 0 (zeroed)
   }
+  kv_word = arena.alloc<int>(1);
   logits = arena.alloc<float>(std::max(T.vocab, C.vocab));
   dbg_logits = arena.alloc<float>((size_t)na * C.vocab);
   tickets = arena.alloc<unsigned>(64);
@@ -1328,6 +1366,54 @@ Engine::~Engine() {
   if (stream) cudaStreamDestroy(stream);
 }
 
+// The talker cache as the kv_*.cu kernels see it: rows' positions end at
+// pos[seq * pos_stride] (null: pos0).
+KvArgs Engine::kv_args(const KvView& kv, int seqs, int max_pages, const int* pos, int pos_stride,
+                       int pos0) {
+  KvArgs c{};
+  const int pages = bt.cap && kv.pool == bt.tkv.pool ? bt.pages * bt.cap : max_pages;
+  c.g = KvGeom{pages, seqs, max_pages, cfg.talker.layers, kv.kv_heads, kv.page_shift, cache.kv_bits};
+  c.pool = reinterpret_cast<unsigned char*>(kv.pool);
+  c.table = const_cast<int*>(kv.page_table);
+  c.lengths = const_cast<int*>(pos);
+  c.len_stride = pos_stride;
+  c.len_add = pos ? 1 : pos0 + 1;
+  c.work = kv_word;
+  return c;
+}
+
+// QK-norm, RoPE and storing of the projected rows in B.qkv, then attention of
+// B.q into B.attn (decode_step_layer_on_stream / prefill_forward's attention).
+void Engine::kv_attention(DevStack& S, StackBufs& B, const KvArgs& c, const KvRows& r, int layer,
+                          const int* halt, int halt_stride) {
+  const StackCfg& k = S.c;
+  KvPrep p{B.qkv, S.qkv_w, k.q_heads, S.q_g[layer], S.k_g[layer], k.eps, S.rope_cos, S.rope_sin,
+           B.q,   layer,   halt,      halt_stride};
+  QCK(launch_kv_prep(c, r, p, stream));
+  KvAttend a{};
+  a.q = KvTensor{B.q, S.q_out, kKvDim};
+  a.out = KvTensor{B.attn, S.q_out, kKvDim};
+  a.type = KV_F32;
+  a.q_heads = k.q_heads;
+  a.scale = 1.0f / std::sqrt((float)k.head_dim);
+  a.window = cache.window;
+  a.sinks = cache.sinks;
+  a.layer = layer;
+  a.halt = halt;
+  a.halt_stride = halt_stride;
+  QCK(launch_kv_attend(c, r, a, stream));
+  launches += 2;
+}
+
+void Engine::check_kv() {
+  if (!kv_form()) return;
+  int e = 0;
+  QCK(cudaMemcpy(&e, kv_word, sizeof(int), cudaMemcpyDeviceToHost));
+  if (!e) return;
+  QCK(cudaMemset(kv_word, 0, sizeof(int)));
+  fail(QTTS_ERR_DEVICE_STATE, "cache attention reported status " + std::to_string(e));
+}
+
 // Decoder layers over M rows at positions pos0.. (prefill_forward, decode.rs:1077-1298).
 void Engine::stack_rows(DevStack& S, StackBufs& B, const KvView& kv, int M, int pos0,
                         const int* halt) {
@@ -1337,12 +1423,18 @@ void Engine::stack_rows(DevStack& S, StackBufs& B, const KvView& kv, int M, int 
   for (int l = 0; l < c.layers; ++l) {
     linear(S.wqkv[l], B.x, c.hidden, S.in_g[l], c.eps, B.qkv, S.qkv_w, nullptr, 0, nullptr, M,
            S.qkv_w, c.hidden, EPI_STORE, halt);
+    if (&S == &talker && kv_form()) {
+      const int pages = (int)((max_cache_steps + (1u << kv.page_shift) - 1) >> kv.page_shift);
+      kv_attention(S, B, kv_args(kv, 1, pages, nullptr, 0, pos0 + M - 1),
+                   KvRows{nullptr, nullptr, 1, M, M, pos0 + M, 1}, l, halt, 0);
+    } else {
     QkPrepArgs qa{B.qkv, S.q_g[l], S.k_g[l], c.eps, S.rope_cos, S.rope_sin, kv, l, pos0, M,
                   c.q_heads, B.q, halt};
     QCK(launch_qk_prep(qa, stream));
     AttnPrefillArgs pa{B.q, kv, l, pos0, M, c.q_heads, scale, B.attn, halt};
     QCK(launch_attn_prefill(pa, stream));
     launches += 2;
+    }
     linear(S.wo[l], B.attn, S.q_out, nullptr, 0.f, B.h1, c.hidden, B.x, c.hidden, nullptr, M,
            c.hidden, S.q_out, EPI_RESID, halt);
     linear(S.wgu[l], B.h1, c.hidden, S.post_g[l], c.eps, B.act, c.intermediate, nullptr, 0,
@@ -1373,7 +1465,13 @@ void Engine::stack_step(DevStack& S, StackBufs& B, const KvView& kv, const int* 
     // before this layer's QKV), except for layer 0 of a CodePredictor group
     // whose QKV row came from the table: the preceding head wrote B.x.
     o.resid_early = !(l == 0 && qkv0_given);
-    if (fuse_attn_o && attn_o_fusable(da, o)) {
+    if (&S == &talker && kv_form()) {
+      const int pages = (int)((max_cache_steps + (1u << kv.page_shift) - 1) >> kv.page_shift);
+      kv_attention(S, B, kv_args(kv, 1, pages, pos_ptr, 1, pos_const),
+                   KvRows{nullptr, nullptr, 1, 1, 1, 0, 0}, l, halt, 0);
+      linear(S.wo[l], B.attn, S.q_out, nullptr, 0.f, B.h1, c.hidden, B.x, c.hidden, nullptr, 1,
+             c.hidden, S.q_out, EPI_RESID, halt, o.resid_early);
+    } else if (fuse_attn_o && attn_o_fusable(da, o)) {
       if (&S == &cp) da.page0 = 0;  // the CodePredictor cache is one page (page 0)
       o.trace_id = trace_tag("attn+o+resid", c.hidden, S.q_out);
       QCK(launch_attn_o(da, o, stream));  // attention inside the O projection's staging
@@ -1674,6 +1772,7 @@ void Engine::sync_state() {
     if (e) fail(QTTS_ERR_DEVICE_STATE, "tensor-core projection pipeline timed out (stage " +
                                            std::to_string(e) + ")");
   }
+  check_kv();
 }
 
 // Enqueues up to n frames (fewer if EOS stops the loop on the device) and
@@ -1804,7 +1903,7 @@ void Engine::ensure_batch() {
   // talker KV: cap sequences x pages each; page table row b = its pages
   bt.tkv = tkv;
   bt.pages = (int)((mcs + (1u << tkv.page_shift) - 1) >> tkv.page_shift);
-  bt.tkv.pool = arena.alloc<__nv_bfloat16>((size_t)(tkv.page_stride * bt.pages * cap));
+  bt.tkv.pool = alloc_talker_pool(bt.pages * cap);
   {
     std::vector<int> pt((size_t)bt.pages * cap);
     for (size_t i = 0; i < pt.size(); ++i) pt[i] = (int)i;
@@ -1852,6 +1951,11 @@ void Engine::batch_stack_step(DevStack& S, StackBufs& B, const KvView& kv, int p
     if (!(l == 0 && qkv0_given))  // else: rows of the precomputed table, written by the heads
       blinear(S.wqkv[l], B.x, c.hidden, S.in_g[l], c.eps, B.qkv, S.qkv_w, nullptr, 0, nullptr,
               nb, S.qkv_w, c.hidden, EPI_STORE);
+    constexpr int kStride = (int)(sizeof(SeqState) / sizeof(int));
+    if (&S == &talker && kv_form()) {
+      kv_attention(S, B, kv_args(kv, nb, pt_stride, pos_ptr, kStride, pos_const),
+                   KvRows{nullptr, nullptr, nb, nb, 1, 0, 0}, l, &bt.st[0].halt, kStride);
+    } else {
     AttnDecodeArgs da{};
     da.qkv = B.qkv;
     da.q_gamma = S.q_g[l];
@@ -1869,12 +1973,13 @@ void Engine::batch_stack_step(DevStack& S, StackBufs& B, const KvView& kv, int p
     da.halt = &bt.st[0].halt;
     da.qkv_ld = S.qkv_w;
     da.out_ld = S.q_out;
-    da.pos_stride = (int)(sizeof(SeqState) / sizeof(int));
-    da.halt_stride = (int)(sizeof(SeqState) / sizeof(int));
+    da.pos_stride = kStride;
+    da.halt_stride = kStride;
     da.pt_stride = pt_stride;
     da.batch = nb;
     QCK(launch_attn_decode(da, stream));
     ++launches;
+    }
     blinear(S.wo[l], B.attn, S.q_out, nullptr, 0.f, B.h1, c.hidden, B.x, c.hidden, nullptr, nb,
             c.hidden, S.q_out, EPI_RESID);
     blinear(S.wgu[l], B.h1, c.hidden, S.post_g[l], c.eps, B.act, c.intermediate, nullptr, 0,
@@ -1951,7 +2056,7 @@ void Engine::batch_head(int role, int group, const float* x, const SampleCfg& c,
 // One frame for nb sequences: CodePredictor positions 0 and 1 (its 2-row
 // prefill, as two decode steps), head 0, groups 1..14, then unless last the
 // talker step and its token (same order as enqueue_frame).
-void Engine::enqueue_batch_frame(const SampleKey& k, int nb) {
+void Engine::enqueue_batch_frame(const SampleKey& k, int nb, const KvView& view) {
   const StackCfg& T = cfg.talker;
   const StackCfg& C = cfg.cp;
   const size_t H = T.hidden;
@@ -1975,20 +2080,20 @@ void Engine::enqueue_batch_frame(const SampleKey& k, int nb) {
     batch_head(ROLE_CP_GROUP, g, bt.cb.x, k.s, 1.0f, nb);
   }
   if (!k.last) {
-    batch_stack_step(talker, bt.tb, bt.tkv, bt.pages, &bt.st[0].talker_pos, 0, nb);
+    batch_stack_step(talker, bt.tb, view, bt.pages, &bt.st[0].talker_pos, 0, nb);
     batch_head(ROLE_TALKER_STEP, 0, bt.tb.x, k.t, k.penalty, nb);
   }
 }
 
-cudaGraphExec_t Engine::batch_graph(const SampleKey& k, int nb) {
-  auto key = std::make_pair(k, nb);
+cudaGraphExec_t Engine::batch_graph(const SampleKey& k, int nb, const KvView& view, bool takes) {
+  auto key = std::make_pair(k, takes ? -nb : nb);
   auto it = batch_graphs.find(key);
   if (it != batch_graphs.end()) return it->second;
   cudaGraph_t g = nullptr;
   const size_t before = launches;
   QCK(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
   try {
-    enqueue_batch_frame(k, nb);
+    enqueue_batch_frame(k, nb, view);
   } catch (...) {
     cudaStreamEndCapture(stream, &g);
     if (g) cudaGraphDestroy(g);
@@ -2004,6 +2109,17 @@ cudaGraphExec_t Engine::batch_graph(const SampleKey& k, int nb) {
   QCK(e);
   batch_graphs[key] = exec;
   return exec;
+}
+
+// The state that a prefill left (sequence, CodePredictor prefix, trailing rows)
+// into batch slot b.
+void Engine::store_slot(int b, int ntr) {
+  const size_t H = cfg.talker.hidden;
+  QCK(cudaMemcpyAsync(bt.st + b, st, sizeof(SeqState), cudaMemcpyDeviceToDevice, stream));
+  QCK(cudaMemcpyAsync(bt.cp_prefix + (size_t)b * 2 * H, cp_prefix_target(),
+                      2 * H * sizeof(float), cudaMemcpyDeviceToDevice, stream));
+  QCK(cudaMemcpyAsync(bt.trailing + (size_t)b * (max_cache_steps + 1) * H, trailing,
+                      (size_t)ntr * H * sizeof(float), cudaMemcpyDeviceToDevice, stream));
 }
 
 void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
@@ -2026,7 +2142,6 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
   const size_t G = cfg.cp.groups;
   if (cap_per_request < (size_t)o0.max_frames * G) invalid("codes_out capacity too small");
   ensure_batch();
-  const size_t H = cfg.talker.hidden;
   // prefill each request into its slot (the single-sequence path on the slot's KV view)
   const KvView saved = tkv;
   QCK(cudaEventRecord(bt.ev[0], stream));
@@ -2039,11 +2154,7 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
       tkv.page_table = bt.tkv.page_table + (size_t)b * bt.pages;
       begin(P, ntr, opts[b]);
       tkv = saved;
-      QCK(cudaMemcpyAsync(bt.st + b, st, sizeof(SeqState), cudaMemcpyDeviceToDevice, stream));
-      QCK(cudaMemcpyAsync(bt.cp_prefix + (size_t)b * 2 * H, cp_prefix_target(),
-                          2 * H * sizeof(float), cudaMemcpyDeviceToDevice, stream));
-      QCK(cudaMemcpyAsync(bt.trailing + (size_t)b * (max_cache_steps + 1) * H, trailing,
-                          (size_t)ntr * H * sizeof(float), cudaMemcpyDeviceToDevice, stream));
+      store_slot(b, ntr);
     }
   } catch (const QttsError& err) {
     tkv = saved;
@@ -2055,6 +2166,14 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
     tkv = saved;
     throw;
   }
+  run_batch(nb, o0, bt.tkv, false, codes_out, cap_per_request, frames_out, ended_out);
+}
+
+// Frames of nb prefilled slots until every one has ended or has max_frames.
+void Engine::run_batch(int nb, const qtts_generate_options& o0, const KvView& view, bool takes,
+                       int32_t* codes_out, size_t cap_per_request, size_t* frames_out,
+                       int32_t* ended_out) {
+  const size_t G = cfg.cp.groups;
   SampleKey full{talker_cfg(o0), sub_cfg(o0), o0.repetition_penalty, 0};
   SampleKey last = full;
   last.last = 1;
@@ -2063,8 +2182,8 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
   // graph (debugging aid: launch errors surface at the launch that caused them)
   const char* eg = std::getenv("QTTS_BATCH_EAGER");
   const bool eager = eg && eg[0] == '1';
-  cudaGraphExec_t gf = !eager && max_frames > 1 ? batch_graph(full, nb) : nullptr;
-  cudaGraphExec_t gl = eager ? nullptr : batch_graph(last, nb);
+  cudaGraphExec_t gf = !eager && max_frames > 1 ? batch_graph(full, nb, view, takes) : nullptr;
+  cudaGraphExec_t gl = eager ? nullptr : batch_graph(last, nb, view, takes);
   size_t done = 0;
   last_launches = 0;
   QCK(cudaEventRecord(bt.ev[1], stream));
@@ -2074,12 +2193,12 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
     for (size_t i = 0; i < burst; ++i) {
       const bool is_last = done + i + 1 >= max_frames;
       if (eager) {
-        enqueue_batch_frame(is_last ? last : full, nb);
+        enqueue_batch_frame(is_last ? last : full, nb, view);
         QCK(cudaStreamSynchronize(stream));
         continue;
       }
       QCK(cudaGraphLaunch(is_last ? gl : gf, stream));
-      last_launches += batch_nodes[std::make_pair(is_last ? last : full, nb)];
+      last_launches += batch_nodes[std::make_pair(is_last ? last : full, takes ? -nb : nb)];
     }
     done += burst;
     QCK(cudaMemcpyAsync(bt.st_host, bt.st, sizeof(SeqState) * nb, cudaMemcpyDeviceToHost,
@@ -2112,6 +2231,7 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
   int tc_e = 0;
   QCK(cudaMemcpy(&tc_e, tc_err, sizeof(int), cudaMemcpyDeviceToHost));
   if (tc_e) fail(QTTS_ERR_DEVICE_STATE, "tensor-core projection pipeline timed out");
+  check_kv();
   last_frames = 0;
   for (int b = 0; b < nb; ++b) {
     const SeqState& s = bt.st_host[b];
@@ -2132,6 +2252,100 @@ void Engine::generate_batch(const std::vector<std::vector<uint32_t>>& ids,
     if (ended_out) ended_out[b] = s.halt ? 1 : 0;
     last_frames += f;
   }
+}
+
+// ---- takes: one prompt, several seeds ---------------------------------------
+void Engine::ensure_takes() {
+  if (bt.takes.table) return;
+  KvArgs& c = bt.takes;
+  c.g = KvGeom{bt.pages * bt.cap, bt.cap, bt.pages, cfg.talker.layers, cfg.talker.kv_heads,
+               bt.tkv.page_shift, cache.kv_bits};
+  c.pool = reinterpret_cast<unsigned char*>(bt.tkv.pool);
+  c.lengths = arena.alloc<int>(bt.cap);
+  c.len_stride = 1;
+  c.refs = arena.alloc<int>(c.g.pages);
+  c.work = arena.alloc<int>(kv_work_ints(c.g));
+  c.table = arena.alloc<int>((size_t)bt.pages * bt.cap);
+}
+
+// The prompt is prefilled once into take 0; the others fork its pages (full ones
+// are shared, the last one is copied) and draw their first token from the same
+// logits with their own seeds. Frames then run as a batch's do.
+void Engine::generate_takes(const uint32_t* ids, size_t n, const qtts_generate_options& o,
+                            const std::vector<uint64_t>& seeds, int32_t* codes_out,
+                            size_t cap_per_take, size_t* frames_out, int32_t* ended_out) {
+  const int nb = (int)seeds.size();
+  if (nb < 1 || nb > kBatchCap) invalid("takes must be in [1, " + std::to_string(kBatchCap) + "]");
+  validate(o);
+  if (cap_per_take < (size_t)o.max_frames * cfg.cp.groups) invalid("codes_out capacity too small");
+  ensure_batch();
+  ensure_takes();
+  int ntr = 0;
+  QCK(cudaEventRecord(bt.ev[0], stream));
+  const int P = prepare(ids, n, 0, o.speaker, o.language, nullptr, &ntr);
+  if ((size_t)P + o.max_frames > max_cache_steps)
+    fail(QTTS_ERR_CACHE_FULL, "requested " + std::to_string(P + o.max_frames) +
+                                  " cache steps but engine was loaded for " +
+                                  std::to_string(max_cache_steps));
+  KvArgs& c = bt.takes;
+  QCK(cudaMemsetAsync(c.table, 0xff, (size_t)c.g.max_pages * c.g.seqs * sizeof(int), stream));
+  QCK(cudaMemsetAsync(c.lengths, 0, c.g.seqs * sizeof(int), stream));
+  QCK(cudaMemsetAsync(c.refs, 0, (size_t)c.g.pages * sizeof(int), stream));
+  KvList list;
+  list.n = 1;
+  list.a[0] = 0;
+  list.b[0] = P;
+  QCK(launch_kv_resize(c, list, stream));
+  KvView view = bt.tkv;
+  view.page_table = c.table;
+  const KvView saved = tkv;
+  qtts_generate_options first = o;
+  first.seed = seeds[0];
+  tkv = view;
+  try {
+    begin(P, ntr, first);
+  } catch (...) {
+    tkv = saved;
+    throw;
+  }
+  tkv = saved;
+  store_slot(0, ntr);
+  for (int b = 1; b < nb; ++b) {
+    SeqState s{};
+    s.semantic = -1;
+    s.talker_pos = P;
+    s.prefill_len = P;
+    s.n_trailing = ntr;
+    s.rng_kind = o.rng;
+    s.rng_state = seeds[b] ^ kSeedXor;
+    s.rng_seed = seeds[b];
+    h2d(st, &s, sizeof s);
+    talker_head(ROLE_TALKER_PREFILL, tb.x + (size_t)(P - 1) * cfg.talker.hidden, talker_cfg(o), 1.0f,
+                nullptr, cp_prefix_target());
+    store_slot(b, ntr);
+  }
+  list.n = nb - 1;
+  for (int b = 1; b < nb; ++b) {
+    list.a[b - 1] = 0;
+    list.b[b - 1] = b;
+  }
+  QCK(launch_kv_fork(c, list, stream));
+  list.n = nb;
+  for (int b = 0; b < nb; ++b) {
+    list.a[b] = b;
+    list.b[b] = P + (int)o.max_frames;
+  }
+  QCK(launch_kv_resize(c, list, stream));
+  int e = 0;
+  QCK(cudaMemcpyAsync(&e, c.work, sizeof e, cudaMemcpyDeviceToHost, stream));
+  stream_sync();
+  if (e) {
+    QCK(cudaMemset(c.work, 0, sizeof e));
+    fail(QTTS_ERR_DEVICE_STATE, "page management reported status " + std::to_string(e));
+  }
+  run_batch(nb, o, view, true, codes_out, cap_per_take, frames_out, ended_out);
+  // no stream of an earlier generation may continue: take 0 ended this one
+  seq_ended = true;
 }
 
 void Engine::read_codes(size_t from, size_t to, int32_t* out) {
@@ -2200,13 +2414,14 @@ void finish_generation(Engine& e, int32_t* codes_out, size_t cap, size_t* frames
   if (ended) *ended = e.seq_ended ? 1 : 0;
 }
 
-int32_t load_engine(const char* dir, int32_t device, size_t mcs, qtts_engine** out) {
+int32_t load_engine(const char* dir, int32_t device, const qtts_cache_options& cache,
+                    qtts_engine** out) {
   return guard([&] {
     need(dir, "model_dir");
     need(out, "out");
     *out = nullptr;
     auto h = std::make_unique<qtts_engine>();
-    h->e = std::make_unique<Engine>(dir, device, mcs);
+    h->e = std::make_unique<Engine>(dir, device, cache);
     *out = h.release();
   });
 }
@@ -2272,7 +2487,7 @@ void qtts_text_stream_options_default(qtts_text_stream_options* o) {
 }
 
 int32_t qtts_engine_load(const char* dir, int32_t device, qtts_engine** out) {
-  return load_engine(dir, device, 512, out);
+  return load_engine(dir, device, {512, 16, 0, 0}, out);
 }
 
 int32_t qtts_engine_load_with_max_frames(const char* dir, int32_t device, size_t max_frames,
@@ -2281,12 +2496,26 @@ int32_t qtts_engine_load_with_max_frames(const char* dir, int32_t device, size_t
     qtts::last_error() = "max_frames must be non-zero";
     return QTTS_ERR_INVALID_INPUT;
   }
-  return load_engine(dir, device, 256 + max_frames, out);
+  return load_engine(dir, device, {256 + max_frames, 16, 0, 0}, out);
 }
 
 int32_t qtts_engine_load_with_options(const char* dir, int32_t device, size_t mcs,
                                       qtts_engine** out) {
-  return load_engine(dir, device, mcs, out);
+  return load_engine(dir, device, {mcs, 16, 0, 0}, out);
+}
+
+void qtts_cache_options_default(qtts_cache_options* o) {
+  if (!o) return;
+  *o = qtts_cache_options{512, 16, 0, 0};
+}
+
+int32_t qtts_engine_load_with_cache(const char* dir, int32_t device,
+                                    const qtts_cache_options* cache, qtts_engine** out) {
+  if (!cache) {
+    qtts::last_error() = "cache must not be null";
+    return QTTS_ERR_INVALID_INPUT;
+  }
+  return load_engine(dir, device, *cache, out);
 }
 
 void qtts_engine_destroy(qtts_engine* e) { delete e; }
@@ -2411,6 +2640,23 @@ int32_t qtts_generate_codes_batch_from_ids(qtts_engine* h, const uint32_t* ids,
     }
     std::vector<qtts_generate_options> o(opts, opts + batch);
     e.generate_batch(reqs, o, codes_out, cap_per_request, frames_out, ended_out);
+  });
+}
+
+int32_t qtts_generate_codes_takes_from_ids(qtts_engine* h, const uint32_t* ids, size_t n,
+                                           const qtts_generate_options* o, const uint64_t* seeds,
+                                           size_t takes, int32_t* codes_out, size_t cap_per_take,
+                                           size_t* frames_out, int32_t* ended_out) {
+  return guard([&] {
+    Engine& e = engine_of(h);
+    need(o, "options");
+    need(seeds, "seeds");
+    need(codes_out, "codes_out");
+    if (n) need(ids, "content_ids");
+    if (takes == 0) qtts::invalid("takes must be non-zero");
+    if (takes > 4096) qtts::invalid("too many takes");
+    e.generate_takes(ids, n, *o, std::vector<uint64_t>(seeds, seeds + takes), codes_out,
+                     cap_per_take, frames_out, ended_out);
   });
 }
 
@@ -2778,8 +3024,8 @@ int32_t qtts_talker_decode_step_static(qtts_engine* h, const float* input, size_
     // step activations, each 64-float aligned: x, qkv, attention, h1, MLP
     auto up = [](size_t n) { return (n + 63) / 64 * 64; };
     const size_t nx = up(H), nqkv = up(S.qkv_w), nattn = up(S.q_out), nh1 = up(H),
-                 nact = up(c.intermediate);
-    const size_t need_bytes = (nx + nqkv + nattn + nh1 + nact) * sizeof(float);
+                 nact = up(c.intermediate), nq = e.kv_form() ? up(S.q_out) : 0;
+    const size_t need_bytes = (nx + nqkv + nattn + nh1 + nact + nq) * sizeof(float);
     if (need_bytes > kStaticScratchBytes)
       qtts::invalid("talker step needs " + std::to_string(need_bytes) +
                     " bytes of activations; the static array holds " +
@@ -2791,6 +3037,7 @@ int32_t qtts_talker_decode_step_static(qtts_engine* h, const float* input, size_
     B.attn = B.qkv + nqkv;
     B.h1 = B.attn + nattn;
     B.act = B.h1 + nh1;
+    B.q = B.act + nact;
     e.h2d(B.x, input, H * 4);
     e.st_host->talker_pos = (int)offset;
     e.st_host->halt = 0;

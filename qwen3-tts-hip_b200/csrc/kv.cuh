@@ -44,6 +44,9 @@ __device__ __forceinline__ KvPlace kv_place(const KvArgs& c, const KvRows& r, in
     if (before >= r.groups || row < __ldg(r.row_start + before)) return at;
     at.group = before;
     back = __ldg(r.row_start + before + 1) - row;
+  } else if (r.one_group) {
+    at.group = 0;
+    back = r.rows - row;
   } else {
     if (row >= r.groups) return at;
     at.group = row;
@@ -178,13 +181,26 @@ __device__ __forceinline__ uint32_t kv_quantise8(const float (&x)[8], float* sca
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const float s = kv_scale_of(m);
   *scale = s;
-  uint32_t w = 0x88888888u;
-  if (s > 0.f) {  // else all zeros, or a marked group
-    const float inv = s >= 1.1754944e-38f ? 1.0f / s : __int_as_float(0x7f800000);
-    w = 0u;
+  if (!(s > 0.f)) return 0x88888888u;  // all zeros, or a marked group
+  uint32_t w = 0u;
+  if (s > 1e-30f) {
+    // t = x / s to two roundings, |t| <= 7.02. Added to 1.5 * 2^23 + 8 it rounds to
+    // an integer whose low four bits are the code; only a t next to a half, where
+    // the exact quotient may lie on the other side, goes the long way below.
+    const float inv = 1.0f / s;
+    float far = 0.f;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) w |= kv_code_of(x[d], s, inv) << (4 * d);
+    for (int d = 0; d < 8; ++d) {
+      const float t = x[d] * inv, v = t + 12582920.0f;
+      w |= (__float_as_uint(v) & 15u) << (4 * d);
+      far = fmaxf(far, fabsf(t - (v - 12582920.0f)));
+    }
+    if (far < 0.4999f) return w;
+    w = 0u;
   }
+  const float inv = s >= 1.1754944e-38f ? 1.0f / s : __int_as_float(0x7f800000);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) w |= kv_code_of(x[d], s, inv) << (4 * d);
   return w;
 }
 

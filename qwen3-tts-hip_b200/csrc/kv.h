@@ -32,6 +32,7 @@ struct KvRows {
   const int* seqs;
   const int* row_start;
   int groups, rows, max_rows, max_length;
+  int one_group;  // with null row_start: all rows are group 0
 };
 
 enum KvType : int { KV_F32 = 0, KV_BF16 = 1 };
@@ -64,6 +65,21 @@ cudaError_t launch_kv_tiles(const KvArgs& c, const KvRows& r, const KvAttend& a,
                             cudaStream_t stream);
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream);
+
+// QK-RMSNorm and RoPE of projected rows [q | k | v]: q to q_out (fp32), k and v
+// stored as launch_kv_append does.
+struct KvPrep {
+  const float* qkv;        // [rows][ld]
+  int ld, q_heads;
+  const float *q_gamma, *k_gamma;  // [128]
+  float eps;
+  const float *rope_cos, *rope_sin;  // [positions][64]
+  float* q_out;            // [rows][q_heads * 128]
+  int layer;
+  const int* halt;         // as KvAttend
+  int halt_stride;
+};
+cudaError_t launch_kv_prep(const KvArgs& c, const KvRows& r, const KvPrep& p, cudaStream_t stream);
 
 struct KvList {
   int n;

@@ -81,7 +81,7 @@ qtts::KvRows rows_of(const qtts_kv_cache* c, const qtts_kv_rows* r) {
   if (!r->seqs && r->groups > c->seqs)
     invalid("rows.groups exceeds the cache's sequences and rows.seqs is null");
   qtts::KvRows k{r->seqs, r->row_start, r->groups, r->groups ? r->rows : 0, r->max_rows,
-                 r->max_length};
+                 r->max_length, 0};
   if (k.max_rows == 0 || k.max_rows > k.rows) k.max_rows = k.row_start ? k.rows : 1;
   return k;
 }

@@ -105,6 +105,64 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
+// The engine's projected rows: a half-warp per (row, q head / k head / v head),
+// lane l of it dims 8 l .. 8 l + 7, so RoPE's partner dim (64 on) is in lane l ^ 8.
+__global__ void __launch_bounds__(kRowThreads) k_kv_prep(KvArgs c, KvRows r, KvPrep p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const long long warp = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
+  const int kvh = c.g.kv_heads, heads = p.q_heads + 2 * kvh, per_row = (heads + 1) / 2;
+  const int row = (int)(warp / per_row);
+  if (row >= r.rows) return;
+  const int j = 2 * (int)(warp - (long long)row * per_row) + (lane >> 4);
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (j < heads) kv_load8(p.qkv, (long long)row * p.ld + (long long)j * kKvDim + 8 * l, KV_F32, x);
+  const KvPlace at = kv_place(c, r, row, true);
+  if (!at.ok || (p.halt && __ldcg(p.halt + (long long)at.group * p.halt_stride))) return;
+  const bool is_q = j < p.q_heads, is_v = j >= p.q_heads + kvh;
+  float ss = 0.f;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) ss += x[d] * x[d];
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = rsqrtf(ss / (float)kKvDim + p.eps);
+  float y[8], o[8];
+  const float* gamma = (is_q ? p.q_gamma : p.k_gamma) + 8 * l;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) y[d] = x[d] * inv * __ldg(gamma + d);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) o[d] = __shfl_xor_sync(0xffffffffu, y[d], 8);
+  const long long rope = (long long)at.pos * 64 + 8 * (l & 7);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    const float cs = __ldg(p.rope_cos + rope + d), sn = __ldg(p.rope_sin + rope + d);
+    const float v = l < 8 ? y[d] * cs - o[d] * sn : y[d] * cs + o[d] * sn;
+    if (!is_v) x[d] = v;
+  }
+  float s = 0.f;
+  const uint32_t codes = c.g.bits == 4 ? kv_quantise8(x, &s) : 0u;  // every lane takes part
+  if (j >= heads) return;
+  if (is_q) {
+    kv_store8(p.q_out, ((long long)row * p.q_heads + j) * kKvDim + 8 * l, KV_F32, x);
+    return;
+  }
+  const int page = kv_page(c, at.seq, at.pos >> c.g.shift);
+  if (page < 0) {
+    kv_bad(c);
+    return;
+  }
+  const int prow = at.pos & ((1 << c.g.shift) - 1);
+  unsigned char* t = c.pool + kv_tile_at(c.g, page, p.layer, is_v, j - p.q_heads - (is_v ? kvh : 0));
+  if (c.g.bits == 16) {
+    kv_store8(t + prow * 2 * kKvDim, 8 * l, KV_BF16, x);
+    return;
+  }
+  *reinterpret_cast<uint32_t*>(t + prow * kKvCodeBytes + kv_code_word_at(8 * l)) = codes;
+  if ((l & 3) == 0)
+    *(reinterpret_cast<__nv_bfloat16*>(t + kv_scale_at(c.g, prow)) + (l >> 2)) = __float2bfloat16_rn(s);
+}
+
 template <bool READ>
 cudaError_t rows_op(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                     const KvTensor& v, int type, cudaStream_t stream) {
@@ -124,6 +182,12 @@ cudaError_t launch_kv_append(const KvArgs& c, const KvRows& r, int layer, const 
 cudaError_t launch_kv_read(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                            const KvTensor& v, int type, cudaStream_t stream) {
   return rows_op<true>(c, r, layer, k, v, type, stream);
+}
+cudaError_t launch_kv_prep(const KvArgs& c, const KvRows& r, const KvPrep& p, cudaStream_t stream) {
+  if (r.rows == 0) return cudaSuccess;
+  const int per_row = (p.q_heads + 2 * c.g.kv_heads + 1) / 2;
+  const long long ctas = ((long long)r.rows * per_row * 32 + kRowThreads - 1) / kRowThreads;
+  return launch(k_kv_prep, dim3((unsigned)ctas), dim3(kRowThreads), 0, stream, c, r, p);
 }
 // Few rows per sequence: the kernel that gives each its own CTA or cluster and
 // streams the cache once per row; more: tiles of rows on the tensor cores.

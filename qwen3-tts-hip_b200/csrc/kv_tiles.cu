@@ -144,8 +144,8 @@ __device__ __forceinline__ bool row_by_row(int seen) {
 // The group of blockIdx.x: its rows and sequence. Same checks as kv_place.
 __device__ __forceinline__ bool group_rows(const KvArgs& c, const KvRows& r, int group, int* seq,
                                            int* begin, int* end, int* len) {
-  *begin = r.row_start ? __ldg(r.row_start + group) : group;
-  *end = r.row_start ? __ldg(r.row_start + group + 1) : group + 1;
+  *begin = r.row_start ? __ldg(r.row_start + group) : r.one_group ? 0 : group;
+  *end = r.row_start ? __ldg(r.row_start + group + 1) : r.one_group ? r.rows : group + 1;
   if (*begin < 0 || *end > r.rows || *begin >= *end) {
     // rows outside the tensor; an empty group is in order
     if (threadIdx.x == 0 && *begin != *end) kv_bad(c);

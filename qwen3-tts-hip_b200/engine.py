@@ -68,6 +68,11 @@ class _StreamOptions(C.Structure):
     _fields_ = [("text_lookahead_tokens", C.c_uint32), ("left_context_frames", C.c_uint32)]
 
 
+class _CacheOptions(C.Structure):
+    _fields_ = [("max_cache_steps", C.c_size_t), ("kv_bits", C.c_int32), ("window", C.c_int32),
+                ("sinks", C.c_int32)]
+
+
 class _TextStreamOptions(C.Structure):
     _fields_ = [("min_start_tokens", C.c_uint32), ("min_resume_tokens", C.c_uint32),
                 ("flush_on_punctuation", C.c_int32), ("left_context_frames", C.c_uint32)]
@@ -108,6 +113,8 @@ SIGNATURES = {
     "qtts_engine_load": (C.c_int32, [C.c_char_p, C.c_int32, C.POINTER(_P)]),
     "qtts_engine_load_with_max_frames": (C.c_int32, [C.c_char_p, C.c_int32, C.c_size_t, C.POINTER(_P)]),
     "qtts_engine_load_with_options": (C.c_int32, [C.c_char_p, C.c_int32, C.c_size_t, C.POINTER(_P)]),
+    "qtts_cache_options_default": (None, [C.POINTER(_CacheOptions)]),
+    "qtts_engine_load_with_cache": (C.c_int32, [C.c_char_p, C.c_int32, C.POINTER(_CacheOptions), C.POINTER(_P)]),
     "qtts_engine_destroy": (None, [_P]),
     "qtts_engine_get_info": (C.c_int32, [_P, C.POINTER(_Info)]),
     "qtts_decode_codes": (C.c_int32, [_P, _I32, C.c_size_t, _F, C.c_size_t, _SZ]),
@@ -117,6 +124,7 @@ SIGNATURES = {
     "qtts_codec_stream_destroy": (None, [_P]),
     "qtts_generate_codes_from_ids": (C.c_int32, [_P, _U32, C.c_size_t, C.POINTER(_Options), _I32, C.c_size_t, _SZ, _I32]),
     "qtts_generate_codes_batch_from_ids": (C.c_int32, [_P, _U32, _SZ, C.c_size_t, C.POINTER(_Options), _I32, C.c_size_t, _SZ, _I32]),
+    "qtts_generate_codes_takes_from_ids": (C.c_int32, [_P, _U32, C.c_size_t, C.POINTER(_Options), C.POINTER(C.c_uint64), C.c_size_t, _I32, C.c_size_t, _SZ, _I32]),
     "qtts_generate_voice_clone_codes_from_ids": (C.c_int32, [_P, _U32, C.c_size_t, _F, C.POINTER(_Options), _I32, C.c_size_t, _SZ, _I32]),
     "qtts_generate_codes_from_rows": (C.c_int32, [_P, _F, C.c_size_t, _F, C.c_size_t, _F, C.POINTER(_Options), _I32, C.c_size_t, _SZ, _I32]),
     "qtts_prepare_inputs_from_ids": (C.c_int32, [_P, _U32, C.c_size_t, C.c_size_t, C.c_char_p, C.c_char_p, _F, _SZ, _F, _SZ, _F]),
@@ -196,6 +204,11 @@ class EngineOptions:
     """EngineOptions (generation.rs:25-38)."""
     device: int = 0
     max_cache_steps: int = DEFAULT_MAX_CACHE_STEPS
+    # How the talker's cache is kept (qtts_cache_options): 16 or 4 bits; a window
+    # of positions that stay visible (0: all) and first positions that always do.
+    kv_bits: int = 16
+    kv_window: int = 0
+    kv_sinks: int = 0
 
 
 @dataclass
@@ -338,8 +351,14 @@ class HipTtsEngine:
     @classmethod
     def load_with_options(cls, model_dir, options: EngineOptions) -> "HipTtsEngine":
         h = C.c_void_p()
-        _check(lib().qtts_engine_load_with_options(str(model_dir).encode(), int(options.device),
-                                                   int(options.max_cache_steps), C.byref(h)))
+        if (options.kv_bits, options.kv_window, options.kv_sinks) == (16, 0, 0):
+            _check(lib().qtts_engine_load_with_options(str(model_dir).encode(), int(options.device),
+                                                       int(options.max_cache_steps), C.byref(h)))
+        else:
+            co = _CacheOptions(int(options.max_cache_steps), int(options.kv_bits),
+                               int(options.kv_window), int(options.kv_sinks))
+            _check(lib().qtts_engine_load_with_cache(str(model_dir).encode(), int(options.device),
+                                                     C.byref(co), C.byref(h)))
         return cls(h, model_dir)
 
     def close(self) -> None:
@@ -402,6 +421,26 @@ class HipTtsEngine:
             res.append(GeneratedCodes(out[b * cap: b * cap + n].tolist(), int(frames[b]),
                                       bool(ended[b])))
         return res
+
+    def generate_codes_takes_from_ids(self, content_ids: Sequence[int], seeds: Sequence[int],
+                                      options: Optional[GenerateOptions] = None
+                                      ) -> List[GeneratedCodes]:
+        """Up to 16 takes of one prompt, one per seed (``options.seed`` is not
+        used): the prompt is prefilled once and the takes share its cache
+        pages. Equal to a batch of that many copies of the request."""
+        options = options or GenerateOptions(decode_audio=False)
+        ids = _ids(content_ids)
+        sd = (C.c_uint64 * max(1, len(seeds)))(*[int(s) & ((1 << 64) - 1) for s in seeds])
+        cap = max(1, options.max_frames) * self.code_groups
+        n = len(seeds)
+        out = np.zeros(max(1, n) * cap, dtype=np.int32)
+        frames = np.zeros(max(1, n), dtype=np.uintp)
+        ended = np.zeros(max(1, n), dtype=np.int32)
+        _check(lib().qtts_generate_codes_takes_from_ids(
+            self._h, ids.ctypes.data_as(_U32), ids.size, C.byref(options._c()), sd, n,
+            out.ctypes.data_as(_I32), cap, frames.ctypes.data_as(_SZ), ended.ctypes.data_as(_I32)))
+        return [GeneratedCodes(out[t * cap: t * cap + int(frames[t]) * self.code_groups].tolist(),
+                               int(frames[t]), bool(ended[t])) for t in range(n)]
 
     def generate_voice_clone_codes_from_ids(self, content_ids, speaker_embedding,
                                             options: Optional[GenerateOptions] = None) -> GeneratedCodes:

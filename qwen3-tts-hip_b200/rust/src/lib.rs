@@ -96,6 +96,15 @@ pub mod ffi {
     }
 
     #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct qtts_cache_options {
+        pub max_cache_steps: usize,
+        pub kv_bits: i32,
+        pub window: i32,
+        pub sinks: i32,
+    }
+
+    #[repr(C)]
     #[derive(Clone, Copy, Debug, Default)]
     pub struct qtts_text_stream_options {
         pub min_start_tokens: u32,
@@ -179,6 +188,10 @@ pub mod ffi {
         pub fn qtts_engine_load_with_options(model_dir: *const c_char, device: i32,
                                              max_cache_steps: usize,
                                              out: *mut *mut qtts_engine) -> i32;
+        pub fn qtts_cache_options_default(out: *mut qtts_cache_options);
+        pub fn qtts_engine_load_with_cache(model_dir: *const c_char, device: i32,
+                                           cache: *const qtts_cache_options,
+                                           out: *mut *mut qtts_engine) -> i32;
         pub fn qtts_engine_destroy(engine: *mut qtts_engine);
         pub fn qtts_engine_get_info(engine: *const qtts_engine, out: *mut qtts_engine_info) -> i32;
         pub fn qtts_decode_codes(engine: *mut qtts_engine, codes: *const i32, n_codes: usize,
@@ -200,6 +213,13 @@ pub mod ffi {
                                                   lengths: *const usize, batch: usize,
                                                   opts: *const qtts_generate_options,
                                                   codes_out: *mut i32, cap_per_request: usize,
+                                                  frames_out: *mut usize,
+                                                  ended_out: *mut i32) -> i32;
+        pub fn qtts_generate_codes_takes_from_ids(engine: *mut qtts_engine,
+                                                  content_ids: *const u32, n_ids: usize,
+                                                  options: *const qtts_generate_options,
+                                                  seeds: *const u64, takes: usize,
+                                                  codes_out: *mut i32, cap_per_take: usize,
                                                   frames_out: *mut usize,
                                                   ended_out: *mut i32) -> i32;
         pub fn qtts_generate_voice_clone_codes_from_ids(engine: *mut qtts_engine,

@@ -157,7 +157,7 @@ def test_python_class_refuses_host_tensors(pkg):
 def test_structs_match_the_rust_binding():
     from test_rust_binding import _c_struct_fields, _rust_struct_fields
 
-    for name in ("qtts_kv_cache", "qtts_kv_rows"):
+    for name in ("qtts_kv_cache", "qtts_kv_rows", "qtts_cache_options"):
         assert _c_struct_fields(name) == _rust_struct_fields(name), name
 
 
@@ -282,3 +282,20 @@ def test_oracle_pages_stay_consistent():
                 c.compact()
             named = [p for r in c.table for p in r if p >= 0]
             assert [named.count(p) for p in range(len(c.refs))] == c.refs
+
+
+def test_engine_cache_options(pkg, tmp_path):
+    from qwen3_tts_hip_b200.engine import _CacheOptions
+
+    o = _CacheOptions()
+    pkg.lib().qtts_cache_options_default(C.byref(o))
+    assert (o.max_cache_steps, o.kv_bits, o.window, o.sinks) == (512, 16, 0, 0)
+    e = pkg.EngineOptions()
+    assert (e.max_cache_steps, e.kv_bits, e.kv_window, e.kv_sinks) == (512, 16, 0, 0)
+    for args, words in (((0, 128, 8), "kv_bits"), ((0, 128, 4, -1), "window"),
+                        ((0, 128, 4, 8, -1), "sinks"), ((0, 128, 4, 0, 3), "sinks need"),
+                        ((0, 0, 4), "max_cache_steps")):
+        with pytest.raises(pkg.InvalidInput, match=words):
+            pkg.HipTtsEngine.load_with_options(tmp_path, pkg.EngineOptions(*args))
+    h = C.c_void_p()
+    refused(pkg, pkg.lib().qtts_engine_load_with_cache(b"/tmp", 0, None, C.byref(h)), "cache")
