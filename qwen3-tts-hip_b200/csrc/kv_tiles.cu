@@ -169,11 +169,20 @@ __device__ __forceinline__ bool group_rows(const KvArgs& c, const KvRows& r, int
   return true;
 }
 
-// 4 bits: 64 positions of a block in a loader thread's registers. K and V:
-// row krow + 8 i, the word of dims 8 kch .. and (bf16, low half) its scale.
+// 4 bits: 64 positions of a block in a loader thread's registers: for K and V,
+// of rows r and r + 32 a quarter of the codes (word g: dims 32 g + 8 t ..) and
+// the row's four scales.
 struct Codes {
-  uint32_t k[8], ks[8], v[8], vs[8];
+  uint4 k[2], v[2];
+  uint2 ks[2], vs[2];
 };
+// In what order a chunk of eight dims is kept, in Q, K and V alike: fp16 operands
+// made of codes come in pairs (d, d + 4), and undoing that would cost four
+// permutes a word. The output's columns are put back in order as they are stored.
+template <int BITS>
+__device__ __forceinline__ constexpr int chunk_dim(int i) {
+  return BITS == 16 ? i : (i >> 1) + 4 * (i & 1);
+}
 
 template <int REGS, bool MORE>
 __device__ __forceinline__ void set_registers() {
@@ -240,7 +249,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_seen;  // what the loaders met (kOdd ..)
   __shared__ int s_dead;  // a wait ran out
-  __shared__ float s_top[2][kRowsM], s_sum[2][kRowsM];
+  __shared__ float s_top[2][Fm::pair ? 1 : kRowsM], s_sum[2][Fm::pair ? 1 : kRowsM];
+  __shared__ float s_down[Fm::qk16 ? Fm::rows : 1];
 
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -315,7 +325,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // before: its product was issued before, and products run in order
         auto scores = [&](int wg, int j) {
           const int g = base + j, s = g % ST;
-          if (!wait(&b.kfull[s], g / ST)) return false;
+          // (a pair's second product follows one that has waited)
+          if ((!Fm::pair || wg == 0) && !wait(&b.kfull[s], g / ST)) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -336,7 +347,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // first: nothing to add to; n: how many products of this group came before
         auto values = [&](int wg, int j, bool first, int n) {
           const int g = base + j, s = g % ST;
-          if (!wait(&b.vfull[s], g / ST) || !wait(&b.pfull[wg], n)) return false;
+          if ((!Fm::pair || wg == 0) && !wait(&b.vfull[s], g / ST)) return false;
+          if (!wait(&b.pfull[wg], n)) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -471,62 +483,63 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       } else {
         int held = -1;
         constexpr int U = KEYS / 64;  // units of 64 positions per block
+        // this thread: rows row and row + 32 of a unit, quarter t. Neighbouring lanes
+        // take rows four apart, so that their swizzled stores meet in no bank.
+        const int t = lt & 3, row = (lt >> 5) * 8 + ((lt >> 3) & 3) + 4 * ((lt >> 2) & 1);
         auto load = [&](Codes& x, int u) {
           const int j = u / U, pc0 = 4 * (u % U), p0 = w.block_pos(j);
           if (u % (U * w.kHeld) == 0) w.refill(c, seq, j, held);
-          const unsigned char* from = kbase + krow * 64 + kv_code_word_at(8 * kch);
-          const unsigned char* from_s = kbase + (kKvCodeBytes << c.g.shift) + krow * 8 + 2 * (kch >> 2);
 #pragma unroll
-          for (int qu = 0; qu < 4; ++qu) {
-            const int page = __shfl_sync(0xffffffffu, held, w.held_lane(j, pc0 + qu));
-            const int p = p0 + 16 * (pc0 + qu);
-            const long long at = max(page, 0) * page_bytes;
-            const unsigned char* src = from + at + (p & mask) * 64;
-            const unsigned char* src_s = from_s + at + (p & mask) * 8;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool ok = page >= 0 && p + krow + 8 * h <= w.last;
-              const int i = 2 * qu + h;
-              x.k[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(src + 512 * h)) : 0u;
-              x.v[i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(src + v_off + 512 * h)) : 0u;
-              x.ks[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(src_s + 64 * h)) : 0u;
-              x.vs[i] = ok ? __ldcg(reinterpret_cast<const uint16_t*>(src_s + v_off + 64 * h)) : 0u;
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int pr = 16 * pc0 + row + 32 * h, p = p0 + pr;
+            const int page = __shfl_sync(0xffffffffu, held, w.held_lane(j, pr >> 4));
+            const unsigned char* tile = kbase + max(page, 0) * page_bytes;
+            const unsigned char* src = tile + (p & mask) * kKvCodeBytes + 16 * t;
+            const unsigned char* src_s = tile + (kKvCodeBytes << c.g.shift) + (p & mask) * 2 * kKvGroups;
+            const bool ok = page >= 0 && p <= w.last;
+            const uint4 none = make_uint4(0u, 0u, 0u, 0u);  // with scales of 0
+            x.k[h] = ok ? __ldcg(reinterpret_cast<const uint4*>(src)) : none;
+            x.v[h] = ok ? __ldcg(reinterpret_cast<const uint4*>(src + v_off)) : none;
+            x.ks[h] = ok ? __ldcg(reinterpret_cast<const uint2*>(src_s)) : make_uint2(0u, 0u);
+            x.vs[h] = ok ? __ldcg(reinterpret_cast<const uint2*>(src_s + v_off)) : make_uint2(0u, 0u);
           }
         };
-        // Eight codes (one word) times their scale, in fp16, dims in order.
-        auto put = [&](uint8_t* dst, uint32_t x, uint32_t s16, int any, int big) {
-          const float s = __uint_as_float(s16 << 16);
-          seen |= (s <= 4096.f ? 0 : kOdd) | (s != 0.f ? any : 0) | (s >= 0.00048828125f ? big : 0);
-          const __half2 sc = __half2half2(__float2half_rn(s));
-          uint32_t o[4];  // pair i: nibbles i and i + 4
+        // Four words of a row times their scales, in fp16: (64 + code) - 72, exact, then
+        // the product, exact for the scales that row_by_row lets pass.
+        unsigned top_k = 0u, top_v = 0u;  // largest scales (bf16 bits; negative and NaN are large)
+        auto put = [&](uint8_t* dst, int r, const uint4& x, const uint2& s4, unsigned& top) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t u = ((x >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
-            const __half2 n =
-                __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
-            const __half2 v = __hmul2(n, sc);
-            o[i] = *reinterpret_cast<const uint32_t*>(&v);
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t word = g == 0 ? x.x : g == 1 ? x.y : g == 2 ? x.z : x.w;
+            const uint32_t sw = g < 2 ? s4.x : s4.y;
+            const uint32_t s16 = g & 1 ? sw >> 16 : sw & 0xffffu;
+            top = max(top, s16);
+            const __half2 sc = __half2half2(__float2half_rn(__uint_as_float(s16 << 16)));
+            uint32_t o[4];  // pair i: nibbles i and i + 4
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t y = i >= 2 ? word >> 8 : word;
+              const uint32_t n = ((i & 1 ? y : y * 16u) & 0x00f000f0u) | 0x54005400u;
+              const __half2 v =
+                  __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&n), __floats2half2_rn(-72.f, -72.f)), sc);
+              o[i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            *reinterpret_cast<uint4*>(dst + (g >> 1) * (KEYS * 128) + swz(r, 4 * (g & 1) + t)) =
+                make_uint4(o[0], o[1], o[2], o[3]);
           }
-          *reinterpret_cast<uint4*>(dst) =
-              make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
-                         __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
         };
         auto store = [&](const Codes& x, int u) {
-          const int g = base + u / U, s = g % ST;
-          const int at = at0 + u % U * (64 * 128);
+          const int g = base + u / U, s = g % ST, r = u % U * 64 + row;
           const bool opens = u % U == 0, closes = u % U == U - 1;
           if (opens && !wait(&b.kempty[s], g / ST + 1)) return false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            put(sk + s * Fm::kv_bytes + at + 1024 * i, x.k[i], x.ks[i], kAnyK, kBigK);
+          for (int h = 0; h < 2; ++h) put(sk + s * Fm::kv_bytes, r + 32 * h, x.k[h], x.ks[h], top_k);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (closes && lane == 0) mbar_arrive(&b.kfull[s]);
           if (opens && !wait(&b.vempty[s], g / ST + 1)) return false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            put(sv + s * Fm::kv_bytes + at + 1024 * i, x.v[i], x.vs[i], kAnyV, kBigV);
+          for (int h = 0; h < 2; ++h) put(sv + s * Fm::kv_bytes, r + 32 * h, x.v[h], x.vs[h], top_v);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (closes && lane == 0) mbar_arrive(&b.vfull[s]);
@@ -541,6 +554,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (u + 2 < units) load(x, u + 2);
           if (!store(y, u + 1)) break;
         }
+        // bf16 bits: 2^12 is 0x4580, 2^-11 0x3a00
+        seen = (max(top_k, top_v) > 0x4580u ? kOdd : 0) | (top_k ? kAnyK : 0) |
+               (top_k >= 0x3a00u ? kBigK : 0) | (top_v ? kAnyV : 0) | (top_v >= 0x3a00u ? kBigV : 0);
       }
       if (seen) atomicOr(&s_seen, seen);
       base += w.blocks;
@@ -560,48 +576,49 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   unsigned dones = 0;
   for (int t = tile0; more(t); t += tiles) {
     w.tile(t);
-    float q_scale = 1.f;  // what undoes the row's power of two
     {
-      // Q of this thread's row (two threads on one row: half of the dims each)
-      const bool in = rr < w.n;
-      const long long off = (long long)(w.row0 + rr) * a.q.row + (long long)(qh0 + hh) * a.q.head;
-      float up = 1.f;
-      if constexpr (Fm::qk16) {
-        float top = 0.f;
-        if (in)
-#pragma unroll 8
-          for (int d = 0; d < kKvDim; d += 4) {
-            const float4 x = kv_load4(a.q.p, off + d, a.type);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-          }
-        if (top > 0.f && isfinite(top)) {
-          // largest magnitude into [2^8, 2^9); the limits keep both factors normal
-          const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -110), 110);
-          up = __uint_as_float((unsigned)(127 + 8 - e) << 23);
-          q_scale = __uint_as_float((unsigned)(127 - 8 + e) << 23);
-        }
-      }
-      // a negative scale goes into Q, so that masked scores are -inf either way
-      if (a.scale < 0.f) up = -up;
+      // Q: a half-warp per matrix row, 16 lanes of eight dims, four rows in flight.
+      // Rows of the other product, and rows past the end, come as they fall.
+      const int hl = lane & 15;
 #pragma unroll 4
-      for (int ch = Fm::pair ? 0 : 8 * wg; ch < (Fm::pair ? 16 : 8 * wg + 8); ++ch) {
+      for (int i = 2 * warp + (lane >> 4); i < Fm::rows; i += 16) {
+        const int ri = i / heads, hi = i - ri * heads;
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (in) {
-          const float4 y = kv_load4(a.q.p, off + 8 * ch, a.type);
-          const float4 z = kv_load4(a.q.p, off + 8 * ch + 4, a.type);
-          x[0] = y.x * up; x[1] = y.y * up; x[2] = y.z * up; x[3] = y.w * up;
-          x[4] = z.x * up; x[5] = z.y * up; x[6] = z.z * up; x[7] = z.w * up;
+        if (ri < w.n)
+          kv_load8(a.q.p, (long long)(w.row0 + ri) * a.q.row + (long long)(qh0 + hi) * a.q.head + 8 * hl,
+                   a.type, x);
+        float up = 1.f;
+        if constexpr (Fm::qk16) {
+          float top = 0.f;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) top = fmaxf(top, fabsf(x[d]));
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          float down = 1.f;
+          if (top > 0.f && isfinite(top)) {
+            // largest magnitude into [2^8, 2^9); the limits keep both factors normal
+            const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -110), 110);
+            up = __uint_as_float((unsigned)(127 + 8 - e) << 23);
+            down = __uint_as_float((unsigned)(127 - 8 + e) << 23);
+          }
+          if (hl == 0) s_down[i] = down;
         }
+        // a negative scale goes into Q, so that masked scores are -inf either way
+        if (a.scale < 0.f) up = -up;
+        float y[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[d] = x[chunk_dim<BITS>(d)] * up;
         uint4 o[PARTS];
-        split8<Fm::qk16, PARTS>(x, o);
+        split8<Fm::qk16, PARTS>(y, o);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
-          *reinterpret_cast<uint4*>(sq + (Fm::pair ? wg * Fm::q_bytes : 0) +
-                                    (2 * p + (ch >> 3)) * (kRowsM * 128) + swz(m, ch & 7)) = o[p];
+          *reinterpret_cast<uint4*>(sq + (i / kRowsM) * Fm::q_bytes + (2 * p + (hl >> 3)) * (kRowsM * 128) +
+                                    swz(i % kRowsM, hl & 7)) = o[p];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     bar<0, kTileThreads>();
+    const float q_scale = Fm::qk16 ? s_down[mi] : 1.f;  // what undoes the row's power of two
     const int pos = rr < w.n ? w.pos0 + rr : -1;
     // (a scale of 0 stays a positive factor: -inf * 0 is not a number)
     const float f = fmaxf(fabsf(a.scale) * kLog2e * q_scale, 1.2e-38f);
@@ -717,10 +734,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto put = [&](int k, const float (&o)[32], float by, bool none) {
       if (rr >= w.n) return;
 #pragma unroll
-      for (int i = 0; i < 32; i += 4)
-        kv_store4(a.out.p, off + k + i, a.type,
-                  none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                       : make_float4(o[i] * by, o[i + 1] * by, o[i + 2] * by, o[i + 3] * by));
+      for (int i = 0; i < 32; i += 8) {
+        float y[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[chunk_dim<BITS>(d)] = none ? 0.f : o[i + d] * by;
+        kv_store8(a.out.p, off + k + i, a.type, y);
+      }
     };
     if constexpr (Fm::pair) {
 #pragma unroll 1
