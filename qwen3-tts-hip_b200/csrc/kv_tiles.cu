@@ -88,6 +88,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations in one instruction, each rounded as ever.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{ .reg .b64 p, q, r; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mov.b64 r, {%6, %7};"
+      " fma.rn.f32x2 p, p, q, r; mov.b64 {%0, %1}, p; }"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{ .reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5};"
+      " add.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p; }"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
 template <bool HALF>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   if constexpr (!HALF) {
@@ -197,12 +214,15 @@ __device__ __forceinline__ void bar() {
 }
 
 // The row tiles of one CTA, the same for every role.
-template <int KEYS>
+template <int KEYS, bool SPLIT>
 struct Walk {
   static constexpr int kPieces = KEYS / 16;        // a page is at least one piece
   static constexpr int kHeld = 32 / kPieces;       // blocks whose pages a warp holds
   int begin, end, len, rows_per, window, sinks;
-  int row0, n, pos0, last, ns, ws, blocks;
+  int row0, n, pos0, last, ns, ws, blocks, skip;
+  // The CTAs of a cluster share a tile's blocks: [total * rank / split, ..) each.
+  __device__ __forceinline__ static int rank() { return SPLIT ? (int)blockIdx.z : 0; }
+  __device__ __forceinline__ static int split() { return SPLIT ? (int)gridDim.z : 1; }
 
   __device__ __forceinline__ void tile(int t) {
     row0 = begin + t * rows_per;
@@ -213,9 +233,14 @@ struct Walk {
     const KvSpan lo = kv_span(max(pos0, 0), window, sinks), hi = kv_span(max(last, 0), window, sinks);
     ns = (hi.sink_end + KEYS - 1) / KEYS;
     ws = max(lo.first / KEYS, ns);
-    blocks = last < 0 ? 0 : ns + max(0, last / KEYS - ws + 1);
+    const int total = last < 0 ? 0 : ns + max(0, last / KEYS - ws + 1);
+    skip = total * rank() / split();
+    blocks = total * (rank() + 1) / split() - skip;
   }
-  __device__ __forceinline__ int block_pos(int j) const { return (j < ns ? j : j - ns + ws) * KEYS; }
+  __device__ __forceinline__ int block_pos(int j) const {
+    j += skip;
+    return (j < ns ? j : j - ns + ws) * KEYS;
+  }
   // every row sees every position of the block at p0
   __device__ __forceinline__ bool whole(int p0) const {
     return pos0 >= 0 && p0 + KEYS - 1 <= pos0 &&
@@ -233,7 +258,7 @@ struct Walk {
   }
 };
 
-template <int BITS, bool F32>
+template <int BITS, bool F32, bool SPLIT>
 __global__ void __launch_bounds__(kTileThreads, 1)
     k_kv_tiles(const __grid_constant__ CUtensorMap map, KvArgs c, KvRows r, KvAttend a, int chunks,
                int gheads, int rows_per, int tiles) {
@@ -249,7 +274,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_seen;  // what the loaders met (kOdd ..)
   __shared__ int s_dead;  // a wait ran out
-  __shared__ float s_top[2][Fm::pair ? 1 : kRowsM], s_sum[2][Fm::pair ? 1 : kRowsM];
+  __shared__ float s_top[2][kRowsM], s_sum[2][kRowsM];  // a pair: of matrix row [group][m]
   __shared__ float s_down[Fm::qk16 ? Fm::rows : 1];
 
   pdl_wait();
@@ -259,7 +284,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int per_head = a.q_heads / c.g.kv_heads;
   const int heads = min(gheads, per_head - chunk * gheads);
   const int qh0 = head * per_head + chunk * gheads;
-  Walk<KEYS> w;
+  Walk<KEYS, SPLIT> w;
   int seq;
   if (!group_rows(c, r, group, &seq, &w.begin, &w.end, &w.len)) return;
   if (a.halt && __ldcg(a.halt + (long long)group * a.halt_stride)) return;
@@ -307,6 +332,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // done with the tile). `base`: blocks of the tiles before (stages and phases
   // run on). After a wait ran out the tiles that are left are skipped.
   int base = 0;
+  // The end of a tile. CTAs that share it meet twice: between() may read what the
+  // others wrote before, and nothing is written over until all have. A CTA whose
+  // wait ran out keeps meeting the others, with no blocks of its own.
+  bool dead = false;
+  auto begin = [&](int t) {
+    w.tile(t);
+    if (SPLIT && dead) w.blocks = 0;
+  };
+  auto finish = [&](auto&& between) {
+    if constexpr (!SPLIT) {
+      bar<0, kTileThreads>();
+      return s_dead == 0;
+    }
+    cluster_arrive();
+    cluster_wait();
+    dead |= s_dead != 0;
+    between();
+    cluster_arrive();
+    cluster_wait();
+    return true;
+  };
 
   if (warp >= kMmaWarp) {
     // ---- matrix instructions: the warp walks together (its operands stay in
@@ -318,7 +364,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint64_t dq = umma_desc_sw128(sq), dk = umma_desc_sw128(sk),
                    dv = umma_desc_sw128_mn(sv, KEYS * 128);
     for (int t = tile0; more(t); t += tiles) {
-      w.tile(t);
+      begin(t);
       bar<0, kTileThreads>();
       if (warp == kMmaWarp) {
         // S goes to the columns of its softmax group, which held P of the block
@@ -418,8 +464,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
       }
       base += w.blocks;
-      bar<0, kTileThreads>();
-      if (s_dead) break;
+      if (!finish([] {})) break;
     }
     tc_fence_before();
     bar<0, kTileThreads>();
@@ -442,7 +487,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int mask = (1 << c.g.shift) - 1;
     const int at0 = (kch >> 3) * (KEYS * 128) + swz(krow, kch & 7);  // row krow + 8 i: + 1024 i
     for (int t = tile0; more(t); t += tiles) {
-      w.tile(t);
+      begin(t);
       bar<0, kTileThreads>();
       int seen = 0;
       if constexpr (BITS == 16) {
@@ -560,8 +605,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (seen) atomicOr(&s_seen, seen);
       base += w.blocks;
-      bar<0, kTileThreads>();
-      if (s_dead) break;
+      if (!finish([] {})) break;
     }
     bar<0, kTileThreads>();
     return;
@@ -575,7 +619,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t quad = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
   unsigned dones = 0;
   for (int t = tile0; more(t); t += tiles) {
-    w.tile(t);
+    begin(t);
     {
       // Q: a half-warp per matrix row, 16 lanes of eight dims, four rows in flight.
       // Rows of the other product, and rows past the end, come as they fall.
@@ -663,7 +707,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < KEYS; ++i) m4[i & 3] = fmaxf(m4[i & 3], x[i]);
+      for (int i = 4; i < KEYS - 4; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], x[i + k]), x[i + 4 + k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[KEYS - 4 + k]);
       const float bt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
       // the first scores set the maximum; later it moves when exceeded by 2^8
       const bool raise = bt > top + 8.f || (top == -INFINITY && bt > -INFINITY);
@@ -674,15 +722,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sum *= corr;
       }
       const float ref = top == -INFINITY ? 0.f : top;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 s2[2] = {{0.f, 0.f}, {0.f, 0.f}};
       // weights, 32 at a time, stored as P over S: per part KEYS / 2 columns of
       // two values (every score has been read)
 #pragma unroll
       for (int i = 0; i < KEYS; i += 32) {
 #pragma unroll
-        for (int k = i; k < i + 32; ++k) {
-          x[k] = exp2_fast(fmaf(x[k], f, -ref));
-          s4[k & 3] += x[k];
+        for (int k = i; k < i + 32; k += 2) {
+          const float2 z = fma2(make_float2(x[k], x[k + 1]), make_float2(f, f), make_float2(-ref, -ref));
+          x[k] = exp2_fast(z.x);
+          x[k + 1] = exp2_fast(z.y);
+          s2[(k >> 1) & 1] = add2(s2[(k >> 1) & 1], make_float2(x[k], x[k + 1]));
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
@@ -709,7 +759,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_st16(my_s + p * (KEYS / 2) + i / 2, o);
         }
       }
-      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      s2[0] = add2(s2[0], s2[1]);
+      sum += s2[0].x + s2[0].y;
       if (j >= (Fm::pair ? 1 : 2) && __any_sync(0xffffffffu, raise)) {
         float o[32];
 #pragma unroll 1
@@ -731,58 +782,111 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     wait(&b.done, dones);
     tc_fence_after();
     const long long off = (long long)(w.row0 + rr) * a.out.row + (long long)(qh0 + hh) * a.out.head;
-    auto put = [&](int k, const float (&o)[32], float by, bool none) {
-      if (rr >= w.n) return;
+    auto put = [&](int k, const float* o, float by, bool none) {  // eight dims
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        float y[8];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) y[chunk_dim<BITS>(d)] = none ? 0.f : o[i + d] * by;
-        kv_store8(a.out.p, off + k + i, a.type, y);
-      }
+      for (int d = 0; d < 8; ++d) y[chunk_dim<BITS>(d)] = none ? 0.f : o[d] * by;
+      if (rr < w.n) kv_store8(a.out.p, off + k, a.type, y);
     };
-    if constexpr (Fm::pair) {
-#pragma unroll 1
-      for (int k = 0; k < kKvDim; k += 32) {
-        float o[32];
-        if (w.blocks) tmem_ld32(my_o + k, o);
-        tmem_ld_wait();
-        put(k, o, 1.0f / sum, sum == 0.f);
-      }
-    } else {
-      // the groups' statistics meet; each then writes half of the dims
+    // This CTA's share of the row: weights of sum l around `top`, and pieces of 32
+    // dims of O (0 where no product wrote it). A pair's thread holds all dims; else
+    // the groups' statistics meet, and each has half of the dims.
+    const int k0 = Fm::pair ? 0 : 64 * wg, k1 = Fm::pair ? kKvDim : k0 + 64;
+    float l = sum, e0 = 1.f, e1 = 1.f;
+    if (SPLIT || !Fm::pair) {
       s_top[wg][m] = top;
       s_sum[wg][m] = sum;
+    }
+    const int g0 = base & 1;  // the group of block 0
+    const bool has0 = w.blocks > (Fm::pair || g0 == 0 ? 0 : 1), has1 = w.blocks > (g0 == 1 ? 0 : 1);
+    if constexpr (!Fm::pair) {
       bar<1, 2 * kGroup>();
       const float t0 = s_top[0][m], t1 = s_top[1][m];
-      const float both = fmaxf(t0, t1), ref = both == -INFINITY ? 0.f : both;
-      const float e0 = exp2_fast(t0 - ref), e1 = exp2_fast(t1 - ref);
-      const float l = e0 * s_sum[0][m] + e1 * s_sum[1][m];
-      const float il = 1.0f / l;
-      // the O of a group that had no block in this tile was never written
-      const int g0 = base & 1;  // the group of block 0
-      const bool has0 = w.blocks > (g0 == 0 ? 0 : 1), has1 = w.blocks > (g0 == 1 ? 0 : 1);
-#pragma unroll 1
-      for (int k = 64 * wg; k < 64 * wg + 64; k += 32) {
-        float o[32], u[32];
+      top = fmaxf(t0, t1);
+      const float ref = top == -INFINITY ? 0.f : top;
+      e0 = exp2_fast(t0 - ref);
+      e1 = exp2_fast(t1 - ref);
+      l = e0 * s_sum[0][m] + e1 * s_sum[1][m];
+    }
+    auto piece = [&](int k, float (&o)[32]) {
+      if constexpr (Fm::pair) {
+        if (has0) tmem_ld32(my_o + k, o);
+        tmem_ld_wait();
+        if (!has0) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+      } else {
+        float u[32];
         if (has0) tmem_ld32(tm_o + quad + k, o);
         if (has1) tmem_ld32(tm_o + kKvDim + quad + k, u);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = (has0 ? o[i] * e0 : 0.f) + (has1 ? u[i] * e1 : 0.f);
-        put(k, o, il, l == 0.f);
+      }
+    };
+    // With more CTAs on the tile each finishes some of the dims, from the pieces of
+    // all of them in shared memory (where K and V were): [dim][row].
+    float* xch = reinterpret_cast<float*>(sk);
+    static_assert(2 * ST * Fm::kv_bytes >= kKvDim * Fm::rows * 4, "a place for O");
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 32) {
+      float o[32];
+      piece(k, o);
+      if constexpr (!SPLIT) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) put(k + i, o + i, 1.0f / l, l == 0.f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) xch[(k + i) * Fm::rows + mi] = o[i];
+      }
+    }
+    if constexpr (SPLIT && !Fm::pair) {
+      bar<1, 2 * kGroup>();  // both groups have read the statistics
+      if (wg == 0) {
+        s_top[0][m] = top;
+        s_sum[0][m] = l;
       }
     }
     tc_fence_before();
     base += w.blocks;
     ++dones;
-    bar<0, kTileThreads>();
-    if (s_dead) break;
-    const int seen = s_seen;
-    bar<1, 2 * kGroup>();
+    int seen = 0;
+    const bool fine = finish([&] {
+      const float* tops = &s_top[Fm::pair ? wg : 0][m];
+      const float* sums = &s_sum[Fm::pair ? wg : 0][m];
+      float all = top;
+      for (int q = 0; q < w.split(); ++q) all = fmaxf(all, ld_cluster_f32(cluster_map(tops, q)));
+      const float ref = all == -INFINITY ? 0.f : all;
+      auto factor = [&](int q) { return exp2_fast(ld_cluster_f32(cluster_map(tops, q)) - ref); };
+      l = 0.f;
+      for (int q = 0; q < w.split(); ++q) {
+        l = fmaf(factor(q), ld_cluster_f32(cluster_map(sums, q)), l);
+        seen |= __float_as_int(ld_cluster_f32(cluster_map(&s_seen, q)));
+      }
+      const int share = (k1 - k0) / w.split();
+#pragma unroll 1
+      for (int k = k0 + share * w.rank(); k < k0 + share * (w.rank() + 1); k += 8) {
+        float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int q = 0; q < w.split(); ++q) {  // in the order of the positions
+          const uint32_t from = cluster_map(&xch[k * Fm::rows + mi], q);
+          const float by = factor(q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = fmaf(by, ld_cluster_f32(from + 4 * i * Fm::rows), z[i]);
+        }
+        put(k, z, 1.0f / l, l == 0.f);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next tile's copies
+    });
+    if (!fine) break;
+    if constexpr (!SPLIT) {
+      seen = s_seen;
+      bar<1, 2 * kGroup>();
+    }
     if (threadIdx.x == 0) s_seen = 0;  // before the next tile's first bar 0
     if (row_by_row(seen))
-      for (int i = warp; i < w.n * heads; i += 8) {
+      for (int i = warp + 8 * w.rank(); i < w.n * heads; i += 8 * w.split()) {
         const int ri = i / heads;
         if (w.pos0 + ri >= 0) kv_attend_row(c, a, seq, w.pos0 + ri, w.row0 + ri, qh0 + i - ri * heads);
       }
@@ -790,22 +894,52 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   bar<0, kTileThreads>();
 }
 
+constexpr int kMaxSplitLog = 3;  // up to 8 CTAs share a tile
+struct Device {  // what a device gave, asked for once
+  bool ready = false;
+  int clusters[kMaxSplitLog + 1];  // of 2^i CTAs that run at once
+};
+
+cudaLaunchConfig_t launch_config(dim3 grid, int smem, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = grid.z;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
 template <int BITS, bool F32>
 cudaError_t tiles(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStream_t stream) {
-  auto kernel = k_kv_tiles<BITS, F32>;
-  constexpr int smem = Form<BITS, F32>::smem;
+  using Fm = Form<BITS, F32>;
   static std::mutex mu;
-  static bool ready[64] = {};
+  static Device devices[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  cudaLaunchAttribute attr[2];
+  Device& d = devices[dev];
   {
     std::lock_guard<std::mutex> lock(mu);
-    if (!ready[dev]) {
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (!d.ready) {
+      e = cudaFuncSetAttribute(k_kv_tiles<BITS, F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fm::smem);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k_kv_tiles<BITS, F32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fm::smem);
+      for (int i = 1; i <= kMaxSplitLog && e == cudaSuccess; ++i) {
+        cudaLaunchConfig_t cfg = launch_config(dim3(1, 1, 1u << i), Fm::smem, stream, attr);
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&d.clusters[i], k_kv_tiles<BITS, F32, true>, &cfg);
+      }
       if (e != cudaSuccess) return e;
-      ready[dev] = true;
+      d.ready = true;
     }
   }
   CUtensorMap map{};
@@ -813,10 +947,22 @@ cudaError_t tiles(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStrea
     return cudaErrorNotSupported;
   const int group = a.q_heads / c.g.kv_heads;
   const int gheads = std::min(group, kRowsM), chunks = (group + gheads - 1) / gheads;
-  const int rows_per = Form<BITS, F32>::rows / gheads;
+  const int rows_per = Fm::rows / gheads;
   const int n = (r.max_rows + rows_per - 1) / rows_per;
-  return launch(kernel, dim3((unsigned)((long long)n * r.groups), (unsigned)(c.g.kv_heads * chunks)),
-                dim3(kTileThreads), (size_t)smem, stream, map, c, r, a, chunks, gheads, rows_per, n);
+  const long long x = (long long)n * r.groups;
+  const int y = c.g.kv_heads * chunks;
+  // Few tiles: as many CTAs to each as run at once, while a share may have two
+  // blocks. One sequence, 128 bf16 rows at position 8,000 over 4-bit pages: 158 us
+  // with one CTA a tile, 99, 62 and 45 with 2, 4 and 8. A second wave costs more than
+  // sharing gives (4 sequences of 512 rows, 128 tiles: 65 us, shared by 2 92 us), and
+  // with one block a CTA it gives nothing (512 rows of a new prompt: 26 us both).
+  const long long span = a.window ? std::min((long long)a.window + a.sinks + rows_per, kv_capacity(c.g))
+                                  : kv_capacity(c.g);
+  int i = kMaxSplitLog;
+  while (i > 0 && (x * y > d.clusters[i] || span < (2ll * Fm::keys << i))) --i;
+  const auto cfg = launch_config(dim3((unsigned)x, (unsigned)y, 1u << i), Fm::smem, stream, attr);
+  return cudaLaunchKernelEx(&cfg, i ? k_kv_tiles<BITS, F32, true> : k_kv_tiles<BITS, F32, false>, map, c, r, a,
+                            chunks, gheads, rows_per, n);
 }
 
 }  // namespace
