@@ -189,12 +189,17 @@ cudaError_t launch_kv_prep(const KvArgs& c, const KvRows& r, const KvPrep& p, cu
   const long long ctas = ((long long)r.rows * per_row * 32 + kRowThreads - 1) / kRowThreads;
   return launch(k_kv_prep, dim3((unsigned)ctas), dim3(kRowThreads), 0, stream, c, r, p);
 }
-// Few rows per sequence: the kernel that gives each its own CTA or cluster and
-// streams the cache once per row; more: tiles of rows on the tensor cores.
+// Few rows: the kernel that gives each its own CTA or cluster and streams the
+// cache once per row; more: tiles of rows on the tensor cores, which read it once
+// per tile and cost the same for 1 row and for 64. Where they meet (us, steps /
+// tiles, bf16 rows): 64 sequences at 2,000, 16 bits, 1 row 24 / 42, 2 rows 48 / 42,
+// 4 rows 81 / 42; 4 sequences at 1,000, 4 bits, 4 rows 4.3 / 6.0, 8 rows 6.0 / 6.0;
+// one sequence at 4,000, 8 rows 6.2 / 7.5, 16 rows 9.6 / 7.7.
 cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
                              cudaStream_t stream) {
   if (r.rows == 0) return cudaSuccess;
-  return r.max_rows <= 8 ? launch_kv_step(c, r, a, stream) : launch_kv_tiles(c, r, a, stream);
+  const bool few = r.max_rows <= 2 || (r.max_rows <= 8 && r.rows <= 16);
+  return few ? launch_kv_step(c, r, a, stream) : launch_kv_tiles(c, r, a, stream);
 }
 
 }  // namespace qtts

@@ -956,8 +956,9 @@ cudaError_t tiles(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStrea
   // with one CTA a tile, 99, 62 and 45 with 2, 4 and 8. A second wave costs more than
   // sharing gives (4 sequences of 512 rows, 128 tiles: 65 us, shared by 2 92 us), and
   // with one block a CTA it gives nothing (512 rows of a new prompt: 26 us both).
-  const long long span = a.window ? std::min((long long)a.window + a.sinks + rows_per, kv_capacity(c.g))
-                                  : kv_capacity(c.g);
+  long long span = kv_capacity(c.g);
+  if (r.max_length) span = std::min(span, (long long)r.max_length);
+  if (a.window) span = std::min(span, (long long)a.window + a.sinks + rows_per);
   int i = kMaxSplitLog;
   while (i > 0 && (x * y > d.clusters[i] || span < (2ll * Fm::keys << i))) --i;
   const auto cfg = launch_config(dim3((unsigned)x, (unsigned)y, 1u << i), Fm::smem, stream, attr);

@@ -8,8 +8,11 @@ a split of q into 16-bit parts and the exponent's argument. Softmax weights
 are then off by a factor within exp(+-2 e), and the weighted sum of n values by
 another (n + 64) * 2^-23, the 64 for the exponentials, the normalisation and
 the merging of partial results. bf16 outputs add half a step, 2^-8 of the value
-at most (with 2^-16 for weights held in two 16-bit parts):
-  |out - exact| <= max_c |v_c| * (expm1(2 e) + (n + 64) * 2^-23 [+ 2^-16])
+at most, and 2^-11 of the largest value for weights rounded once to fp16: a
+weight is off by at most 2^-11 of itself, so the weighted mean by 2^-11 max |v|
+(below fp16's normal range by 2^-25 at most each, beside a sum of at least 1: the
+2^-23 above per value covers it):
+  |out - exact| <= max_c |v_c| * (expm1(2 e) + (n + 64) * 2^-23 [+ 2^-11])
                    [+ 2^-8 * |exact|].
 """
 import numpy as np
@@ -121,7 +124,7 @@ def check_rows(got, q, groups, filled, layer, window, sinks, scale=128 ** -0.5, 
             e = 144 * 2.0 ** -23 * abs(scale) * mag
             tol = big * (np.expm1(2 * e) + (len(at) + 64) * 2.0 ** -23)
             if got.dtype == BF16:
-                tol = tol[:, None] + 2.0 ** -16 * big[:, None] + 2.0 ** -8 * np.abs(want)
+                tol = tol[:, None] + 2.0 ** -11 * big[:, None] + 2.0 ** -8 * np.abs(want)
             else:
                 tol = tol[:, None]
             bad = np.abs(got64[r] - want) > tol
@@ -212,6 +215,50 @@ def test_rows_counts(pkg, bits, dtype, rows):
     # a hint that is too small costs time, not rows
     out = f.cache.attend(0, q, row_start=starts, max_rows=1, max_length=1)
     check_rows(out, q, [(0, rows + 37, 0, rows), (1, rows, rows, 2 * rows)], f, 0, 0, 0)
+
+
+# few tiles over long caches: CTAs share the positions of a tile, some of them none
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens,rows,kv", [([3001], [40], 1), ([700, 2500, 64, 9], [17, 64, 64, 9], 1),
+                                          ([1500, 40], [300, 40], 2), ([1030], [20], 8)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 3), (33, 200)])
+def test_few_rows_over_long_caches(pkg, bits, dtype, lens, rows, kv, window, sinks):
+    f = Filled(pkg, lens, kv=kv, bits=bits, width=128, seed=sum(lens), layers=1)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    q = rand_q(int(starts[-1]), 2 * kv, dtype)
+    kw = dict(row_start=torch.tensor(starts, dtype=torch.int32, device=DEV), max_rows=max(rows),
+              window=window, sinks=sinks)
+    out = f.cache.attend(0, q, **kw)
+    assert torch.equal(out, f.cache.attend(0, q, **kw))
+    check_rows(out, q, [(s, n, starts[s], starts[s + 1]) for s, n in enumerate(lens)], f, 0, window,
+               sinks)
+    # told of fewer rows, CTAs take more tiles in turn; told of the lengths, fewer share one
+    for more in (dict(max_rows=9), dict(max_length=max(lens))):
+        check_rows(f.cache.attend(0, q, **{**kw, **more}), q,
+                   [(s, n, starts[s], starts[s + 1]) for s, n in enumerate(lens)], f, 0, window, sinks)
+    f.cache.check()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_shared_tiles_agree_on_odd_values(pkg, bits, dtype):
+    """A NaN that some rows of a tile see and others do not, in one CTA's share."""
+    n, rows, window, sinks = 2000, 40, 1200, 5
+    f = Filled(pkg, [n], kv=1, bits=bits, layers=1, seed=8, width=128)
+    p = n - rows - window + 21  # seen by rows 0 to 20
+    pool = f.host.copy()
+    page, r = f.table[0, p // 32], p % 32
+    if bits == 16:
+        pool.view(np.uint16).reshape(-1, 1, 2, 1, 32, 128)[page, 0, 1, 0, r, 5] = 0x7fc0
+    else:
+        pool[page, 0, 1, 0, 32 * 64 + r * 8: 32 * 64 + r * 8 + 2] = np.array([0x7fc0], np.uint16).view(np.uint8)
+    f.cache.pool.copy_(torch.from_numpy(pool.reshape(-1)))
+    q = rand_q(rows, 2, dtype)
+    starts = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    out = f.cache.attend(0, q, window=window, sinks=sinks, row_start=starts)
+    hit = torch.isnan(out)
+    assert hit[:21, :, 5].all() and not hit[21:].any() and not hit[..., 64:].any()
 
 
 def test_rows_wide_window_long(pkg):
