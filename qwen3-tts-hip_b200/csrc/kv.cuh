@@ -125,19 +125,47 @@ __device__ __forceinline__ float4 kv_cached4(const KvArgs& c, int page, int laye
                      (float)((int)((n >> 8) & 15u) - 8) * s, (float)((int)(n >> 12) - 8) * s);
 }
 
+// Eight: one access of 32 (16) bytes where the address allows.
 __device__ __forceinline__ void kv_load8(const void* p, long long off, int type, float (&x)[8]) {
+  if (type == KV_F32) {
+    const float* f = static_cast<const float*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(f) & 31) == 0) {
+      asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]),
+                     "=f"(x[7])
+                   : "l"(f)
+                   : "memory");
+      return;
+    }
+  } else {
+    const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+      unpack8(__ldcg(reinterpret_cast<const uint4*>(b)), x);
+      return;
+    }
+  }
   const float4 a = kv_load4(p, off, type), b = kv_load4(p, off + 4, type);
   x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 __device__ __forceinline__ void kv_store8(void* p, long long off, int type, const float (&x)[8]) {
-  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p) + off;
-  if (type == KV_BF16 && (reinterpret_cast<uintptr_t>(h) & 15) == 0) {
-    __nv_bfloat162 w[4];
+  if (type == KV_F32) {
+    float* f = static_cast<float*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(f) & 31) == 0) {
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(f), "f"(x[0]),
+                   "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                   : "memory");
+      return;
+    }
+  } else {
+    __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p) + off;
+    if ((reinterpret_cast<uintptr_t>(h) & 15) == 0) {
+      __nv_bfloat162 w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(w);
-    return;
+      for (int i = 0; i < 4; ++i) w[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(w);
+      return;
+    }
   }
   kv_store4(p, off, type, make_float4(x[0], x[1], x[2], x[3]));
   kv_store4(p, off + 4, type, make_float4(x[4], x[5], x[6], x[7]));

@@ -335,8 +335,11 @@ __global__ void __launch_bounds__(kCopyThreads) k_copy_pages(KvArgs c, int remap
   }
 }
 
-cudaError_t copy_pages(const KvArgs& c, int remap, cudaStream_t stream) {
-  return launch(k_copy_pages, dim3(148 * 8), dim3(kCopyThreads), 0, stream, c, remap);
+// For at most `copies` pages: a block per piece, up to all that run at once.
+cudaError_t copy_pages(const KvArgs& c, int copies, int remap, cudaStream_t stream) {
+  const long long pieces = (kv_page_bytes(c.g) + kCopyPiece - 1) / kCopyPiece * copies;
+  const unsigned blocks = (unsigned)(pieces < 148 * 8 ? pieces : 148 * 8);
+  return launch(k_copy_pages, dim3(blocks), dim3(kCopyThreads), 0, stream, c, remap);
 }
 
 }  // namespace
@@ -344,12 +347,12 @@ cudaError_t copy_pages(const KvArgs& c, int remap, cudaStream_t stream) {
 cudaError_t launch_kv_resize(const KvArgs& c, const KvList& l, cudaStream_t stream) {
   if (l.n == 0) return cudaSuccess;
   const cudaError_t e = launch(k_resize, dim3(1), dim3(kPlanThreads), 0, stream, c, l);
-  return e != cudaSuccess ? e : copy_pages(c, 0, stream);
+  return e != cudaSuccess ? e : copy_pages(c, l.n, 0, stream);
 }
 cudaError_t launch_kv_fork(const KvArgs& c, const KvList& l, cudaStream_t stream) {
   if (l.n == 0) return cudaSuccess;
   const cudaError_t e = launch(k_fork, dim3(1), dim3(kPlanThreads), 0, stream, c, l);
-  return e != cudaSuccess ? e : copy_pages(c, 0, stream);
+  return e != cudaSuccess ? e : copy_pages(c, l.n, 0, stream);
 }
 cudaError_t launch_kv_drop(const KvArgs& c, const KvList& l, int window, int sinks,
                            cudaStream_t stream) {
@@ -358,7 +361,7 @@ cudaError_t launch_kv_drop(const KvArgs& c, const KvList& l, int window, int sin
 }
 cudaError_t launch_kv_compact(const KvArgs& c, cudaStream_t stream) {
   const cudaError_t e = launch(k_plan_compact, dim3(1), dim3(kPlanThreads), 0, stream, c);
-  return e != cudaSuccess ? e : copy_pages(c, 1, stream);
+  return e != cudaSuccess ? e : copy_pages(c, c.g.pages, 1, stream);
 }
 
 }  // namespace qtts

@@ -8,24 +8,23 @@ namespace qtts {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowBatch = 4;  // pairs of units in flight per warp
+constexpr int kRowBatch = 2;  // pairs of units in flight per warp (store and load of 3,334 rows: 22 us; 4: 23, 8: 29)
 
 // A unit is one row of K or V of one kv head; a half-warp takes it, lane l of it
 // dims 8 l .. 8 l + 7 (one word of codes; four lanes share a scale). A warp has
-// one row's place and up to eight of its units, whose values are on their way
+// one row's place and up to four of its units, whose values are on their way
 // while the place is looked up (three dependent reads). Bound by bytes: every
 // value is read once and written once.
 template <bool READ>
 __global__ void __launch_bounds__(kRowThreads)
-    k_kv_rows(KvArgs c, KvRows r, int layer, KvTensor k, KvTensor v, int type, int per_row) {
+    k_kv_rows(KvArgs c, KvRows r, int layer, KvTensor k, KvTensor v, int type) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, l = lane & 15;
-  const long long warp = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
-  const int row = (int)(warp / per_row);
+  const int row = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
   if (row >= r.rows) return;
   const int units = 2 * c.g.kv_heads;
-  const int u0 = (int)(warp - (long long)row * per_row) * 2 * kRowBatch + (lane >> 4);
+  const int u0 = blockIdx.y * 2 * kRowBatch + (lane >> 4);
   auto tensor_at = [&](int u, long long* off) -> const KvTensor& {
     const bool is_v = u >= c.g.kv_heads;
     const KvTensor& t = is_v ? v : k;
@@ -79,7 +78,8 @@ __global__ void __launch_bounds__(kRowThreads)
       } else if (page >= 0) {
         const float s = __uint_as_float(sc[i] << 16);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) y[d] = (float)((int)((w[i].x >> (4 * d)) & 15u) - 8) * s;
+        for (int d = 0; d < 8; ++d)  // 2^23 + code, less 2^23 + 8: exact, and no conversion
+          y[d] = (__uint_as_float(((w[i].x >> (4 * d)) & 15u) | 0x4b000000u) - 8388616.0f) * s;
       }
       long long off;
       const KvTensor& t = tensor_at(u0 + 2 * i, &off);
@@ -167,10 +167,9 @@ template <bool READ>
 cudaError_t rows_op(const KvArgs& c, const KvRows& r, int layer, const KvTensor& k,
                     const KvTensor& v, int type, cudaStream_t stream) {
   if (r.rows == 0) return cudaSuccess;
-  const int per_row = (2 * c.g.kv_heads + 2 * kRowBatch - 1) / (2 * kRowBatch);
-  const long long ctas = ((long long)r.rows * per_row * 32 + kRowThreads - 1) / kRowThreads;
-  return launch(k_kv_rows<READ>, dim3((unsigned)ctas), dim3(kRowThreads), 0, stream, c, r, layer, k,
-                v, type, per_row);
+  const int per_cta = kRowThreads / 32, per_warp = 2 * kRowBatch;
+  const dim3 grid((unsigned)((r.rows - 1) / per_cta + 1), (unsigned)((2 * c.g.kv_heads - 1) / per_warp + 1));
+  return launch(k_kv_rows<READ>, grid, dim3(kRowThreads), 0, stream, c, r, layer, k, v, type);
 }
 
 }  // namespace
