@@ -8,13 +8,17 @@ namespace qtts {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowBatch = 2;  // pairs of units in flight per warp (store and load of 3,334 rows: 22 us; 4: 23, 8: 29)
+// Pairs of units in flight per warp: 3,334 rows stored and read take 25, 22, 23 and
+// 29 us with 1, 2, 4 and 8 (more warps hide the look-up better than longer ones).
+constexpr int kRowBatch = 2;
 
 // A unit is one row of K or V of one kv head; a half-warp takes it, lane l of it
 // dims 8 l .. 8 l + 7 (one word of codes; four lanes share a scale). A warp has
 // one row's place and up to four of its units, whose values are on their way
-// while the place is looked up (three dependent reads). Bound by bytes: every
-// value is read once and written once.
+// while the place is looked up (three dependent reads). Every value is read once
+// and written once. Measured: 3,334 fp32 rows of 8 kv heads stored in 4 bits and
+// read back, 59 MB in all: 22 us for both, 2.7 TB/s; half of it is the start of two
+// kernels and their chains of dependent reads.
 template <bool READ>
 __global__ void __launch_bounds__(kRowThreads)
     k_kv_rows(KvArgs c, KvRows r, int layer, KvTensor k, KvTensor v, int type) {

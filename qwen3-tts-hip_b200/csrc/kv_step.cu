@@ -3,12 +3,14 @@
 //
 // One CTA (or a cluster of them, each with a share of the positions) serves
 // one row's query heads of one kv head, at most four. A warp takes tiles of 16
-// positions straight from global memory into the registers of the matrix
-// instruction, with no shared memory between:
+// positions from its ring in shared memory into the registers of the matrix
+// instruction:
 //   S^T[16 positions][8] = K[16][128] * Q^T      (K the 16-row operand)
 //   O^T[128 dims][8]    += V^T[128][16] * P^T    (V^T the 16-row operand)
 // The order of the summed index is free, so each lane's 16-byte loads are
-// operand fragments as they are (K) or after one byte permute per pair (V).
+// operand fragments as they are (K) or after one byte permute per pair (V). With
+// one to four query heads per position there is too little to multiply for wider
+// tiles: the instruction is there to save the shuffles of a dot product.
 // The 8 columns are (head t, part 0 or 1) = column 2 t + part: what a bf16
 // operand cannot hold of a query or a weight goes into its second part (and,
 // for fp32 rows, a third one through a second instruction into the same
@@ -29,7 +31,13 @@
 // Rows come by bulk copies into a ring of each warp's own: 16 positions of 16
 // bits (two contiguous pieces of 4 KB) or 32 of 4 bits (four pieces, 4,608
 // bytes) to a slot. What is in flight does not depend on registers or on how
-// many warps an SM holds, which matters most for a few streams.
+// many warps an SM holds, which matters most for a few streams (32 long windowed
+// streams: 104 us with loads into registers, 93 so; 64 4-bit streams 244 and 222).
+//
+// Measured: 32 streams of 16 heads behind a window of 4,096 positions, 16 bits:
+// 93 us, 5.8 TB/s, 88% of what a copy reaches. 64 streams at 7,000 to 8,191, 4 bits:
+// 198 us, 2.9 TB/s, bound by the bit operations. One stream at 512: 8 us, bound by
+// the launch.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
 // CTAs of a cluster through distributed shared memory, both in a fixed order.
