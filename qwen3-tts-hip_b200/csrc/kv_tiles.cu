@@ -390,15 +390,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if ((!Fm::pair || wg == 0) && !wait(&b.kfull[s], g / ST)) return false;
           tc_fence_after();
           if (elect_one()) {
+            // (the small parts first: an addition cuts what lies below the sum's last
+            // bit; 265 fp32 rows against 64 bits: 1.8e-7 off, large parts first 1.2e-6)
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
+            for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
               for (int k = 0; k < 8; ++k)  // halves of 64 dims, four steps of 32 bytes in each
                 umma_bf16(tm_s + wg * Fm::s_cols,
                           dq + (((Fm::pair ? wg * Fm::q_bytes : 0) +
                                  (2 * p + (k >> 2)) * (kRowsM * 128)) >> 4) + 2 * (k & 3),
                           dk + ((s * Fm::kv_bytes + (k >> 2) * (KEYS * 128)) >> 4) + 2 * (k & 3), is,
-                          (p | k) != 0);
+                          p < PARTS - 1 || k != 0);
             if (!Fm::pair || wg == 1) umma_commit(&b.kempty[s]);
             umma_commit(&b.sfull[wg]);
           }
@@ -413,11 +415,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
+            for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
               for (int k = 0; k < KEYS / 16; ++k)
                 umma_16_ts(tm_o + wg * kKvDim, tm_s + wg * Fm::s_cols + p * (KEYS / 2) + 8 * k,
-                           dv + ((s * Fm::kv_bytes + k * 16 * 128) >> 4), io, !first || (p | k) != 0);
+                           dv + ((s * Fm::kv_bytes + k * 16 * 128) >> 4), io, !first || p < PARTS - 1 || k != 0);
             if (!Fm::pair || wg == 1) umma_commit(&b.vempty[s]);
           }
           __syncwarp();
