@@ -1,6 +1,8 @@
 // Storing rows into a paged key / value cache and loading them back.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kv.cuh"
 
@@ -198,9 +200,14 @@ cudaError_t launch_kv_prep(const KvArgs& c, const KvRows& r, const KvPrep& p, cu
 // tiles, bf16 rows): 64 sequences at 2,000, 16 bits, 1 row 24 / 42, 2 rows 48 / 42,
 // 4 rows 81 / 42; 4 sequences at 1,000, 4 bits, 4 rows 4.3 / 6.0, 8 rows 6.0 / 6.0;
 // one sequence at 4,000, 8 rows 6.2 / 7.5, 16 rows 9.6 / 7.7.
-cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& a,
+cudaError_t launch_kv_attend(const KvArgs& c, const KvRows& r, const KvAttend& attend,
                              cudaStream_t stream) {
   if (r.rows == 0) return cudaSuccess;
+  // a window no sequence can outgrow hides nothing, and positions past a table's
+  // end do not exist: within these limits the kernels' sums of them fit 32 bits
+  KvAttend a = attend;
+  if (a.window >= kv_capacity(c.g)) a.window = 0;
+  a.sinks = (int)std::min<long long>(a.sinks, kv_capacity(c.g));
   const bool few = r.max_rows <= 2 || (r.max_rows <= 8 && r.rows <= 16);
   return few ? launch_kv_step(c, r, a, stream) : launch_kv_tiles(c, r, a, stream);
 }

@@ -217,6 +217,19 @@ def test_rows_counts(pkg, bits, dtype, rows):
     check_rows(out, q, [(0, rows + 37, 0, rows), (1, rows, rows, 2 * rows)], f, 0, 0, 0)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1),
+                                          (2 ** 31 - 90, 7), (3, 2 ** 31 - 1)])
+def test_spans_at_the_ends_of_their_type(pkg, bits, rows, window, sinks):
+    f = Filled(pkg, [150], kv=1, bits=bits, layers=1, seed=3)
+    starts = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    for dtype in (F32, BF16):
+        q = rand_q(rows, 2, dtype)
+        out = f.cache.attend(0, q, row_start=starts, window=window, sinks=sinks)
+        check_rows(out, q, [(0, 150, 0, rows)], f, 0, window, sinks)
+
+
 # few tiles over long caches: CTAs share the positions of a tile, some of them none
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("dtype", [F32, BF16])
