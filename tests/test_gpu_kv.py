@@ -230,6 +230,41 @@ def test_spans_at_the_ends_of_their_type(pkg, bits, rows, window, sinks):
         check_rows(out, q, [(0, 150, 0, rows)], f, 0, window, sinks)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_groups_of_unknown_rows(pkg, bits, dtype):
+    rng = np.random.default_rng(7)
+    rows = rng.integers(0, 20, 300)
+    rows[11] = 700  # far more tiles than its share
+    lens = rows + rng.integers(0, 30, 300)
+    f = Filled(pkg, lens.tolist(), kv=1, ps=16, bits=bits, layers=1, seed=2)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    q = rand_q(int(starts[-1]), 2, dtype)
+    out = f.cache.attend(0, q, row_start=torch.tensor(starts, dtype=torch.int32, device=DEV), window=50,
+                         sinks=2)
+    check_rows(out, q, [(s, n, starts[s], starts[s + 1]) for s, n in enumerate(lens)], f, 0, 50, 2)
+    f.cache.check()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_captured_chunks(pkg, bits):
+    """Rows of two sequences captured once; replays follow lengths and rows."""
+    f = Filled(pkg, [900, 300], kv=1, bits=bits, layers=1, width=64, seed=5)
+    starts = torch.tensor([0, 30, 60], dtype=torch.int32, device=DEV)
+    q, out = rand_q(60, 2, BF16), torch.zeros(60, 2, 128, dtype=BF16, device=DEV)
+    f.cache.attend(0, q, row_start=starts, window=400, sinks=3, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        f.cache.attend(0, q, row_start=starts, window=400, sinks=3, out=out)
+    for n0, n1, r0 in ((900, 300, 30), (700, 20, 11), (31, 299, 50)):
+        f.cache.lengths.copy_(torch.tensor([n0, n1], dtype=torch.int32))
+        starts.copy_(torch.tensor([0, r0, 60], dtype=torch.int32))
+        q.copy_(rand_q(60, 2, BF16, n0))
+        g.replay()
+        check_rows(out, q, [(0, n0, 0, r0), (1, n1, r0, 60)], f, 0, 400, 3)
+
+
 # few tiles over long caches: CTAs share the positions of a tile, some of them none
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("dtype", [F32, BF16])
