@@ -192,6 +192,7 @@ int32_t qtts_kv_attend(const qtts_kv_cache* cache, int32_t layer, const qtts_kv_
     if (q_heads > 65535) invalid("q_heads must be at most 65535");
     if (!std::isfinite(scale)) invalid("scale must be finite");
     check_span(window, sinks);
+    if (r.rows && q == out) invalid("out must not overlap q");  // (rows may be read again after others are written)
     a.type = dtype;
     a.q_heads = q_heads;
     a.scale = scale;

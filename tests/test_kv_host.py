@@ -87,7 +87,7 @@ def test_bad_rows_are_refused(pkg, kv, over, words):
     ({"heads": 0}, "q_heads"), ({"scale": float("nan")}, "scale"),
     ({"scale": float("inf")}, "scale"), ({"window": -1}, "window"), ({"sinks": -1}, "sinks"),
     ({"dtype": 2}, "dtype"), ({"q": None}, "q"), ({"out": None}, "out"), ({"q": P + 2}, "aligned"),
-    ({"stride": 1 << 41}, "stride"),
+    ({"stride": 1 << 41}, "stride"), ({"q": P, "out": P}, "overlap"),
 ])
 def test_bad_attend_arguments_are_refused(pkg, kv, over, words):
     refused(pkg, attend(pkg, kv, cache(kv), rows(kv, groups=1, rows=1), **over), words)
