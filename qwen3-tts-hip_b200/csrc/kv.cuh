@@ -73,6 +73,13 @@ __device__ __forceinline__ KvPlace kv_place(const KvArgs& c, const KvRows& r, in
   return at;
 }
 
+// (x & mask) | bits in one instruction (two immediates would make two of it).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+
 // Four consecutive values of a row tensor; 16-byte (8-byte) accesses where the
 // address allows, else one by one.
 __device__ __forceinline__ float4 kv_load4(const void* p, long long off, int type) {

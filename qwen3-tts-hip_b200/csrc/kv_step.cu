@@ -19,8 +19,8 @@
 // parts costs one addition.
 //
 // 4-bit rows: codes become small integers by bit operations, which run at half
-// rate and bound the 4-bit form (an and-or per pair of codes, a shift for half
-// of them). K: each group of 32 dims accumulates apart and its scale multiplies
+// rate and bound the 4-bit form (an and-or per pair of codes, in one instruction:
+// 198 -> 181 us below; a shift for half of them). K: each group of 32 dims accumulates apart and its scale multiplies
 // the fp32 sum. V: the scale multiplies the fp32 weight.
 //   bf16 rows: fp16 operands, a nibble in place in the mantissa of 64.0. K: 64 +
 //   code is used as it is and 72 times the query's sum is taken off the fp32
@@ -36,7 +36,7 @@
 //
 // Measured: 32 streams of 16 heads behind a window of 4,096 positions, 16 bits:
 // 93 us, 5.8 TB/s, 88% of what a copy reaches. 64 streams at 7,000 to 8,191, 4 bits:
-// 198 us, 2.9 TB/s, bound by the bit operations. One stream at 512: 8 us, bound by
+// 181 us, 3.1 TB/s, bound by the bit operations and the arithmetic around them. One stream at 512: 8 us, bound by
 // the launch.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
@@ -97,7 +97,7 @@ __device__ __forceinline__ uint32_t shifted(uint32_t w, int left) {
 // one right shift serves two of them, the left shifts are products.
 __device__ __forceinline__ uint32_t nibbles_64(uint32_t w, int i) {
   const uint32_t x = i >= 2 ? w >> 8 : w;
-  return ((i & 1 ? x : x * 16u) & 0x00f000f0u) | 0x54005400u;
+  return and_or(i & 1 ? x : x * 16u, 0x00f000f0u, 0x54005400u);
 }
 // As code - 8, exact, in fp16 or bf16 (there from 16 + code, mantissa bits 3-6).
 __device__ __forceinline__ uint32_t nibbles_half(uint32_t w, int i) {
@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t nibbles_half(uint32_t w, int i) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, int i) {
-  const uint32_t u = (shifted(w, 3 - 4 * i) & 0x00780078u) | 0x41804180u;
+  const uint32_t u = and_or(shifted(w, 3 - 4 * i), 0x00780078u, 0x41804180u);
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
                                    __nv_bfloat162(__float2bfloat16(24.f), __float2bfloat16(24.f)));
   return *reinterpret_cast<const uint32_t*>(&r);

@@ -33,7 +33,7 @@
 // of 128 positions and 256 matrix rows takes 4,400 clocks, of which the products
 // are 2,050 and the exponentials 2,050 at the units' rates: what bounds it is the
 // chain scores -> maximum -> weights -> product of each group, which the other
-// fills by half. 4 sequences of 100 to 512 rows at 1,000 to 4,000, 4 bits: 91 us,
+// fills by half. 4 sequences of 100 to 512 rows at 1,000 to 4,000, 4 bits: 89 us,
 // the longest tile's chain (96 tiles, 148 SMs).
 //
 // Number forms. 16-bit pages, bf16 rows: Q K^T in bf16 as it is; P in fp16
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t y = i >= 2 ? word >> 8 : word;
-              const uint32_t n = ((i & 1 ? y : y * 16u) & 0x00f000f0u) | 0x54005400u;
+              const uint32_t n = and_or(i & 1 ? y : y * 16u, 0x00f000f0u, 0x54005400u);
               const __half2 v =
                   __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&n), __floats2half2_rn(-72.f, -72.f)), sc);
               o[i] = *reinterpret_cast<const uint32_t*>(&v);
