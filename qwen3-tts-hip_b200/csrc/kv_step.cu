@@ -29,14 +29,14 @@
 //   fp32 rows: code - 8 in bf16 (exact), weight times scale in three parts.
 //
 // Rows come by bulk copies into a ring of each warp's own: 16 positions of 16
-// bits (two contiguous pieces of 4 KB) or 32 of 4 bits (four pieces, 4,608
-// bytes) to a slot. What is in flight does not depend on registers or on how
+// bits (two contiguous pieces of 4 KB) or 32 of 4 bits (4,608 bytes: two pieces
+// with pages of 32 positions, else four or eight, 171 and 181 us below) to a slot. What is in flight does not depend on registers or on how
 // many warps an SM holds, which matters most for a few streams (32 long windowed
 // streams: 104 us with loads into registers, 93 so; 64 4-bit streams 244 and 222).
 //
 // Measured: 32 streams of 16 heads behind a window of 4,096 positions, 16 bits:
 // 93 us, 5.8 TB/s, 88% of what a copy reaches. 64 streams at 7,000 to 8,191, 4 bits:
-// 181 us, 3.1 TB/s, bound by the bit operations and the arithmetic around them. One stream at 512: 8 us, bound by
+// 171 us, 3.3 TB/s, bound by the bit operations and the arithmetic around them. One stream at 512: 8 us, bound by
 // the launch.
 //
 // Statistics, scores and sums are fp32. Warps merge through shared memory,
@@ -152,8 +152,10 @@ struct __align__(16) Slot<16> {
 template <>
 struct __align__(16) Slot<4> {
   static constexpr int unit = 2 * kTile, ring = 2;
-  uint4 k[unit * 4], v[unit * 4];  // 64 bytes a row
-  uint2 ks[unit], vs[unit];
+  uint4 k[unit * 4];  // 64 bytes a row
+  uint2 ks[unit];     // (as in a page of `unit` rows)
+  uint4 v[unit * 4];
+  uint2 vs[unit];
 };
 
 // Operand fragments of the tile at row0 of a slot. (16-bit rows lie 256 bytes
@@ -504,6 +506,10 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas<BITS, F32>)
         const unsigned char* k = kbase + max(pg0, 0) * page_bytes + row * (2 * kKvDim);
         bulk_g2s(p.k, k, sizeof p.k, bar);
         bulk_g2s(p.v, k + v_off, sizeof p.v, bar);
+      } else if (mask + 1 == UNIT) {  // a page's rows and scales in one piece
+        const unsigned char* k = kbase + max(pg0, 0) * page_bytes;
+        bulk_g2s(p.k, k, sizeof p.k + sizeof p.ks, bar);
+        bulk_g2s(p.v, k + v_off, sizeof p.v + sizeof p.vs, bar);
       } else {
         for (int u = 0; u < UNIT; u += piece) {  // pieces of 16 start a page
           const unsigned char* tile = kbase + max(u ? pg1 : pg0, 0) * page_bytes;
