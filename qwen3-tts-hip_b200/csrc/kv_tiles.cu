@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using Fm = Form<BITS, F32>;
   constexpr int PARTS = Fm::parts, KEYS = Fm::keys, ST = Fm::stages;
   extern __shared__ uint8_t tile_smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(tile_smem_raw) + 1023) & ~uintptr_t(1023));
+  // (an offset, not a rounded address: accesses stay known to be to shared memory)
+  uint8_t* smem = tile_smem_raw + (-smem_u32(tile_smem_raw) & 1023u);
   uint8_t* sq = smem;
   uint8_t* sk = sq + Fm::rows / kRowsM * Fm::q_bytes;  // stages of K, then of V
   uint8_t* sv = sk + ST * Fm::kv_bytes;
