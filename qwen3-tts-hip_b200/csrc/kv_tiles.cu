@@ -29,11 +29,11 @@
 // launch).
 //
 // Measured: two prompts of 2,500 to 4,096 bf16 rows behind a window of 2,048, 16
-// heads over 8 kv heads: 163 us, 530 TFLOP/s, a third of the matrix peak. A block
+// heads over 8 kv heads: 155 us, 570 TFLOP/s, a third of the matrix peak. A block
 // of 128 positions and 256 matrix rows takes 4,400 clocks, of which the products
 // are 2,050 and the exponentials 2,050 at the units' rates: what bounds it is the
 // chain scores -> maximum -> weights -> product of each group, which the other
-// fills by half. 4 sequences of 100 to 512 rows at 1,000 to 4,000, 4 bits: 89 us,
+// fills by half. 4 sequences of 100 to 512 rows at 1,000 to 4,000, 4 bits: 88 us,
 // the longest tile's chain (96 tiles, 148 SMs).
 //
 // Number forms. 16-bit pages, bf16 rows: Q K^T in bf16 as it is; P in fp16
@@ -294,8 +294,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = blockIdx.x % r.groups;
-  const int head = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+  // heads first, then groups, then tiles
+  const int per_tile = c.g.kv_heads * chunks, across = (int)(blockIdx.x % per_tile);
+  const int place = (int)(blockIdx.x / per_tile), group = place % r.groups;
+  const int head = across / chunks, chunk = across % chunks;
   const int per_head = a.q_heads / c.g.kv_heads;
   const int heads = min(gheads, per_head - chunk * gheads);
   const int qh0 = head * per_head + chunk * gheads;
@@ -306,9 +308,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   w.rows_per = rows_per;
   w.window = a.window;
   w.sinks = a.sinks;
-  // tiles with more positions first; more row tiles than the launch was told
-  // of are taken in turn
-  const int tile0 = tiles - 1 - (int)(blockIdx.x / r.groups);
+  // tiles with more positions first, of all heads (prompts below: 163 us with each
+  // head's tiles together); more row tiles than the launch was told of are taken in turn
+  const int tile0 = tiles - 1 - place / r.groups;
   auto more = [&](int t) { return (long long)t * rows_per < w.end - w.begin; };
 
   if (threadIdx.x == 0) {
@@ -986,7 +988,7 @@ cudaError_t tiles(const KvArgs& c, const KvRows& r, const KvAttend& a, cudaStrea
   if (a.window) span = std::min(span, (long long)a.window + a.sinks + rows_per);
   int i = kMaxSplitLog;
   while (i > 0 && (x * y > d.clusters[i] || span < (2ll * Fm::keys << i))) --i;
-  const auto cfg = launch_config(dim3((unsigned)x, (unsigned)y, 1u << i), Fm::smem, stream, attr);
+  const auto cfg = launch_config(dim3((unsigned)(x * y), 1u, 1u << i), Fm::smem, stream, attr);
   return cudaLaunchKernelEx(&cfg, i ? k_kv_tiles<BITS, F32, true> : k_kv_tiles<BITS, F32, false>, map, c, r, a,
                             chunks, gheads, rows_per, n);
 }
