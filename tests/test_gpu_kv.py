@@ -582,6 +582,42 @@ def test_captured_steps(pkg, bits):
     c.check()
 
 
+FIRST_IN_A_GRAPH = """
+import torch
+from __graft_entry__ import load_package
+pkg = load_package()
+cs = [pkg.KvCache.allocate(2, 4096, layers=1, kv_heads=1, kv_bits=b) for b in (16, 4)]
+for c in cs:
+    c.resize([0, 1], [700, 90])
+    c.pool.zero_()
+torch.cuda.synchronize()
+out = []
+g = torch.cuda.CUDAGraph()
+starts = torch.tensor([0, 40, 80], dtype=torch.int32, device="cuda")
+qs = [torch.randn(80, 2, 128, device="cuda").to(t) for t in (torch.float32, torch.bfloat16)]
+with torch.cuda.graph(g):  # no kernel of these has run in this process
+    for c in cs:
+        for q in qs:
+            out += [c.attend(0, q, row_start=starts), c.attend(0, q[:2].contiguous())]
+g.replay()
+torch.cuda.synchronize()
+assert all(not t.any() for t in out)
+for c in cs:
+    c.check()
+print("fine")
+"""
+
+
+def test_first_calls_may_be_captured(pkg):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], capture_output=True, text=True,
+                       timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
 def test_repeats_are_bitwise_equal(pkg):
     f = Filled(pkg, [3000, 1000], kv=2, bits=4, layers=1, seed=1)
     for rows in (1, 300):
