@@ -265,6 +265,18 @@ def test_captured_chunks(pkg, bits):
         check_rows(out, q, [(0, n0, 0, r0), (1, n1, r0, 60)], f, 0, 400, 3)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("group", [7, 130])
+def test_more_heads_than_a_tile_has_rows(pkg, bits, dtype, group):
+    f = Filled(pkg, [70, 40], kv=1, bits=bits, layers=1, seed=group)
+    for rows in (1, 19):
+        q = rand_q(2 * rows, group, dtype)
+        starts = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device=DEV)
+        out = f.cache.attend(0, q, row_start=starts, window=30, sinks=2)
+        check_rows(out, q, [(0, 70, 0, rows), (1, 40, rows, 2 * rows)], f, 0, 30, 2)
+
+
 # few tiles over long caches: CTAs share the positions of a tile, some of them none
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("dtype", [F32, BF16])
